@@ -17,6 +17,7 @@ from .api import (  # noqa: F401
     launch_count,
     total_attention,
 )
+from .cache import KVCache4, attention_with_kv_cache, kv_cache_read, kv_cache_write  # noqa: F401
 
 __all__ = [
     "attention",
@@ -30,4 +31,8 @@ __all__ = [
     "attention_cross_token_qk_sum",
     "total_attention",
     "compute_attention_scores",
+    "KVCache4",
+    "kv_cache_write",
+    "kv_cache_read",
+    "attention_with_kv_cache",
 ]

@@ -32,6 +32,7 @@ EXPORTS = [
     "faws_attention_with_col_sum_sequential",
     "faws_attention_with_softmax_col_sum", "faws_attention_cross_token_qk_sum",
     "faws_attention_cross_token_softmax_sum", "faws_attention_cross_token_softmax_sum_buffered",
+    "faws_kv_cache_write", "faws_kv_cache_read", "faws_attention_with_kv_cache", "faws_kv_cache_workspace_bytes",
     "faws_total_attention", "faws_attention_backward", "faws_workspace_bytes", "faws_reduce_ranks", "faws_device_status",
     "faws_selftest_wait_give_up", "faws_last_backend",
     "faws_launch_count", "faws_strerror", "faws_version",
@@ -64,6 +65,16 @@ class Grads(C.Structure):
     _fields_ = [("dout", Tensor), ("dq", Tensor), ("dk", Tensor), ("dv", Tensor)]
 
 
+class KVCache(C.Structure):
+    _fields_ = [("k_codes", C.c_void_p), ("v_codes", C.c_void_p), ("k_scales", C.c_void_p), ("v_scales", C.c_void_p),
+                ("pages", C.c_int32), ("page_size", C.c_int32), ("Hk", C.c_int32), ("D", C.c_int32), ("dtype", C.c_int32)]
+
+
+class CacheBatch(C.Structure):
+    _fields_ = [("page_table", C.c_void_p), ("lengths", C.c_void_p), ("table_stride", C.c_int64), ("B", C.c_int32),
+                ("max_pages", C.c_int32)]
+
+
 _lib = None
 
 
@@ -79,6 +90,7 @@ def load():
     lib = C.CDLL(LIB_PATH)
     PP = C.POINTER(Problem)
     vp, i32, u32, sz = C.c_void_p, C.c_int32, C.c_uint32, C.c_size_t
+    cache = [C.POINTER(KVCache), C.POINTER(CacheBatch)]
     protos = {
         "faws_attention": (i32, [PP, vp]),
         "faws_dropout_mask_bytes": (sz, [PP]),
@@ -96,6 +108,10 @@ def load():
         "faws_attention_cross_token_qk_sum": (i32, [PP, i32, vp, i32, vp, sz, vp]),
         "faws_attention_cross_token_softmax_sum": (i32, [PP, i32, vp, i32, vp, sz, vp]),
         "faws_attention_cross_token_softmax_sum_buffered": (i32, [PP, i32, vp, i32, vp, sz, vp]),
+        "faws_kv_cache_write": (i32, cache + [C.POINTER(Tensor), C.POINTER(Tensor), i32, vp]),
+        "faws_kv_cache_read": (i32, cache + [C.POINTER(Tensor), C.POINTER(Tensor), i32, vp]),
+        "faws_attention_with_kv_cache": (i32, [PP] + cache + [i32, i32, vp, sz, vp]),
+        "faws_kv_cache_workspace_bytes": (sz, [PP]),
         "faws_total_attention": (i32, [PP, vp, vp]),
         "faws_attention_backward": (i32, [PP, C.POINTER(Grads), vp, sz, vp]),
         "faws_workspace_bytes": (sz, [i32, PP, i32]),

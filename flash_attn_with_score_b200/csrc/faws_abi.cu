@@ -443,6 +443,27 @@ bool forward_draws_mask(const faws_problem* p) {
   return p->causal ? 2 * tiles >= 5 * sms : 6 * 2 * sms * ((ctas + sms - 1) / sms) <= 7 * tiles;
 }
 
+// The 4-bit cache and the sequences of a call; `rows` rows of each.
+int validate_cache(const faws_kv_cache* c, const faws_cache_batch* b, int64_t rows) {
+  if (c == nullptr || b == nullptr) return FAWS_EINVAL;
+  if (c->pages <= 0 || c->Hk <= 0 || b->B <= 0 || b->max_pages <= 0 || rows <= 0) return FAWS_EINVAL;
+  if (c->page_size < 16 || c->page_size > 65536 || (c->page_size & (c->page_size - 1)) != 0) return FAWS_EINVAL;
+  if (c->D != 16 && c->D != 32 && c->D != 64 && c->D != 128) return FAWS_EUNSUPPORTED;
+  if (c->dtype != FAWS_FP16 && c->dtype != FAWS_BF16) return FAWS_EUNSUPPORTED;
+  if (b->page_table == nullptr || b->lengths == nullptr || b->table_stride < 0) return FAWS_EINVAL;
+  for (const void* x : {c->k_codes, c->v_codes, c->k_scales, c->v_scales})
+    if (x == nullptr || reinterpret_cast<uintptr_t>(x) % 16 != 0) return FAWS_EINVAL;
+  // a block has 2048 elements of these rows, a grid 2^31 - 1 blocks
+  if ((int64_t)b->B * c->Hk > (int64_t(1) << 40) / (rows * c->D)) return FAWS_EINVAL;
+  return FAWS_OK;
+}
+CacheParams make_cache(const faws_kv_cache* c) {
+  int shift = 0;
+  while ((1 << shift) < c->page_size) ++shift;
+  return {c->k_codes, c->v_codes, c->k_scales, c->v_scales, c->pages, shift, c->Hk, c->D};
+}
+CacheBatch make_batch(const faws_cache_batch* b) { return {b->page_table, b->table_stride, b->lengths, b->B, b->max_pages}; }
+
 size_t split_kv_bytes(const faws_problem* p, int n_splits) {
   return align256((size_t)p->B * p->Hq * n_splits * p->M * 4) +
          align256((size_t)p->B * p->Hq * n_splits * p->M * p->D * 4);
@@ -734,6 +755,63 @@ size_t faws_workspace_bytes(int32_t op, const faws_problem* p, int32_t split) {
     default:
       return 0;
   }
+}
+
+int faws_kv_cache_write(const faws_kv_cache* c, const faws_cache_batch* batch, const faws_tensor* k, const faws_tensor* v,
+                        int32_t rows, void* stream) {
+  const int st = validate_cache(c, batch, rows);
+  if (st != FAWS_OK) return st;
+  if (k == nullptr || v == nullptr || k->ptr == nullptr || v->ptr == nullptr) return FAWS_EINVAL;
+  return launch_cache_write(make_cache(c), make_batch(batch), k, v, rows, c->dtype, static_cast<cudaStream_t>(stream)) == cudaSuccess
+             ? FAWS_OK
+             : FAWS_ECUDA;
+}
+
+int faws_kv_cache_read(const faws_kv_cache* c, const faws_cache_batch* batch, const faws_tensor* k, const faws_tensor* v,
+                       int32_t rows, void* stream) {
+  const int st = validate_cache(c, batch, rows);
+  if (st != FAWS_OK) return st;
+  if (k == nullptr || v == nullptr || k->ptr == nullptr || v->ptr == nullptr) return FAWS_EINVAL;
+  return launch_cache_read(make_cache(c), make_batch(batch), k, v, rows, c->dtype, static_cast<cudaStream_t>(stream)) == cudaSuccess
+             ? FAWS_OK
+             : FAWS_ECUDA;
+}
+
+size_t faws_kv_cache_workspace_bytes(const faws_problem* p) {
+  if (p == nullptr || p->B <= 0 || p->Hq <= 0 || p->Hk <= 0 || p->M <= 0 || p->Hq % p->Hk != 0) return 0;
+  if (p->D != 16 && p->D != 32 && p->D != 64 && p->D != 128) return 0;
+  const int64_t rows = (int64_t)(p->Hq / p->Hk) * p->M;
+  return align256(cache_attn_workspace_bytes(rows > 8 ? 16 : 8, p->D));
+}
+
+int faws_attention_with_kv_cache(const faws_problem* p, const faws_kv_cache* c, const faws_cache_batch* batch,
+                                 int32_t window, int32_t sinks, void* workspace, size_t workspace_bytes, void* stream) {
+  if (p == nullptr || p->Hq <= 0 || p->Hk <= 0 || p->M <= 0 || p->Hq % p->Hk != 0) return FAWS_EINVAL;
+  const int64_t rows = (int64_t)(p->Hq / p->Hk) * p->M;
+  const int st = validate_cache(c, batch, rows);
+  if (st != FAWS_OK) return st;
+  if (p->B != batch->B || p->Hk != c->Hk || p->D != c->D || p->dtype != c->dtype) return FAWS_EINVAL;
+  if (p->q.ptr == nullptr || p->out.ptr == nullptr || window < 0 || sinks < 0 || rows > (1 << 30)) return FAWS_EINVAL;
+  if (workspace == nullptr || workspace_bytes < faws_kv_cache_workspace_bytes(p) || misaligned_ws(workspace)) return FAWS_EWORKSPACE;
+  CacheAttnParams a{};
+  a.cache = make_cache(c);
+  a.batch = make_batch(batch);
+  a.q = p->q.ptr; a.out = p->out.ptr;
+  a.q_sb = p->q.stride_b; a.q_sh = p->q.stride_h; a.q_ss = p->q.stride_s;
+  a.o_sb = p->out.stride_b; a.o_sh = p->out.stride_h; a.o_ss = p->out.stride_s;
+  a.L = p->log_normalizer;
+  a.G = p->Hq / p->Hk; a.M = p->M; a.rows = (int)rows;
+  a.window = window == 0 || window > (1 << 30) ? 1 << 30 : window;
+  a.sinks = sinks > (1 << 30) ? 1 << 30 : sinks;
+  a.sm_scale = p->sm_scale;
+  a.parts = static_cast<float*>(workspace);
+  const cudaError_t e = launch_cache_attn(a, p->dtype, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) {
+    std::fprintf(stderr, "faws: cache attention launch failed: %s\n", cudaGetErrorString(e));
+    return FAWS_ECUDA;
+  }
+  t_last_backend = FAWS_BACKEND_GENERIC;
+  return FAWS_OK;
 }
 
 int faws_reduce_ranks(const float* parts, int32_t n_ranks, int64_t count, float* out, void* stream) {

@@ -202,7 +202,44 @@ struct ScoresOnlyParams {
   float sm_scale;
 };
 
+// The 4-bit cache (faws_kv_cache) and the sequences of a call (faws_cache_batch), for its kernels.
+struct CacheParams {
+  void* k_codes;
+  void* v_codes;
+  void* k_scales;
+  void* v_scales;
+  int pages, page_shift, Hk, D;
+};
+struct CacheBatch {
+  const int32_t* table;    // (B, max_pages), rows `table_stride` apart
+  int64_t table_stride;
+  const int32_t* lengths;  // (B)
+  int B, max_pages;
+};
+struct CacheAttnParams {
+  CacheParams cache;
+  CacheBatch batch;
+  const void* q;
+  void* out;
+  int64_t q_sb, q_sh, q_ss;
+  int64_t o_sb, o_sh, o_ss;
+  float* L;           // (B,Hq,M) or null
+  int G, M, rows;     // rows: G * M, of a kv head
+  int window, sinks;  // at most 2^30
+  float sm_scale;
+  // set by the launcher
+  int row_blocks, grid, min_tiles, vec_out;
+  float* parts;       // workspace
+  int* status;
+};
+
 // Launchers (each returns a cudaError_t from the launch).
+cudaError_t launch_cache_write(const CacheParams& c, const CacheBatch& b, const faws_tensor* k, const faws_tensor* v, int rows,
+                               int dtype, cudaStream_t s);
+cudaError_t launch_cache_read(const CacheParams& c, const CacheBatch& b, const faws_tensor* k, const faws_tensor* v, int rows,
+                              int dtype, cudaStream_t s);
+size_t cache_attn_workspace_bytes(int rows, int D);
+cudaError_t launch_cache_attn(const CacheAttnParams& p, int dtype, cudaStream_t s);  // p.parts = the workspace
 cudaError_t launch_generic_scores_only(const ScoresOnlyParams& p, int dtype, cudaStream_t s);
 bool tc_scores_only_supported(const ScoresOnlyParams& p, int dtype);
 cudaError_t launch_tc_scores_only(const ScoresOnlyParams& p, int dtype, cudaStream_t s);

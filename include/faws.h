@@ -299,6 +299,58 @@ int faws_attention_backward_masked(const faws_problem* p, const faws_grads* g, c
 size_t faws_workspace_bytes(int32_t op, const faws_problem* p, int32_t split);
 
 /*
+ * A paged cache of keys and values in 4 bits, and the operators on it.  No counterpart in the reference.
+ *
+ * A row (one token of one kv head) is cut into groups of min(32, D) neighbouring elements.  A group has a scale s =
+ * bf16(amax / 7) and codes sign(x) floor(|x| / s + 1/2) in -7 .. 7, and stands for s * code.  s is 0 where it would be
+ * below 2^-126; a group that holds an infinity or a NaN reads as NaN throughout.
+ *
+ * The caller owns the four arrays, contiguous and 16-byte aligned: codes of pages * Hk * page_size rows of D / 2 bytes,
+ * scales of as many rows of max(1, D / 32) bf16 numbers.  How codes lie within a row is the library's affair.  Rows that
+ * were never written may hold anything.
+ */
+typedef struct faws_kv_cache {
+  void *k_codes, *v_codes, *k_scales, *v_scales;
+  int32_t pages, page_size; /* page_size: tokens of a page, a power of two, 16 to 65536 */
+  int32_t Hk, D;
+  int32_t dtype;            /* of the rows that are written and read: FAWS_FP16 | FAWS_BF16 */
+} faws_kv_cache;
+
+/*
+ * The sequences of a call.  Position n of sequence b lies in page page_table[b * table_stride + n / page_size].  lengths[b]
+ * counts the tokens of sequence b, those of the call among them: the calls below take `rows` (M) rows per sequence, row m
+ * being position lengths[b] - rows + m (aligned to the end, as causal masks are).  Rows before position 0 are padding.
+ * Both arrays are on the device.  A length below 0 or beyond max_pages * page_size is taken as the nearest bound and a
+ * page outside [0, pages) is not touched; both raise the device's status word (faws_device_status: 2).
+ */
+typedef struct faws_cache_batch {
+  const int32_t* page_table;
+  const int32_t* lengths;
+  int64_t table_stride;
+  int32_t B, max_pages;
+} faws_cache_batch;
+
+/* Quantises the rows of k and v, (B,Hk,rows,D) views, into the cache; padding rows and rows on bad pages are skipped.  The
+ * positions that a call writes are to be in different places: two rows for the same place leave it undefined. */
+int faws_kv_cache_write(const faws_kv_cache* c, const faws_cache_batch* batch, const faws_tensor* k, const faws_tensor* v,
+                        int32_t rows, void* stream);
+
+/* The values of rows of the cache, into k and v, (B,Hk,rows,D) views; padding rows become 0, rows on bad pages NaN. */
+int faws_kv_cache_read(const faws_kv_cache* c, const faws_cache_batch* batch, const faws_tensor* k, const faws_tensor* v,
+                       int32_t rows, void* stream);
+
+/*
+ * Causal attention of the last p->M rows of each sequence over the cache.  Of p: B, Hq, Hk, M, D, dtype, sm_scale, q, out and
+ * log_normalizer ((B,Hq,M) or NULL) are used; the rest is ignored.  window 0: a row sees every key up to its own position;
+ * window > 0: the last `window` of those, and the first `sinks` ones (faws_attention_with_window).  Rows that see nothing (padding, empty
+ * sequences) become 0.  Keys on bad pages are NaN.  Deterministic.  Workspace: faws_kv_cache_workspace_bytes(p), 256-byte
+ * aligned.
+ */
+int faws_attention_with_kv_cache(const faws_problem* p, const faws_kv_cache* c, const faws_cache_batch* batch,
+                                 int32_t window, int32_t sinks, void* workspace, size_t workspace_bytes, void* stream);
+size_t faws_kv_cache_workspace_bytes(const faws_problem* p);
+
+/*
  * Query-split multi-GPU variant: out[i] = parts[0][i] + parts[1][i] + ... in
  * rank order (deterministic).  parts: n_ranks contiguous vectors of `count`
  * floats each, rank-major, in this GPU's own memory (e.g. the landing buffer
@@ -310,8 +362,10 @@ int faws_reduce_ranks(const float* parts, int32_t n_ranks, int64_t count, float*
 /*
  * The tcgen05 kernels bound every wait on an mbarrier (2 s).  A CTA that gives up
  * raises a per-device status word, frees its TMEM and returns; its outputs are then
- * invalid.  This call synchronises the device and returns that word (0 = no give-up,
- * 1 = some wait gave up, -1 = the word could not be read); `reset` != 0 clears it.
+ * invalid.  The cache operators raise it where a page table or a length names what the
+ * cache does not have.  This call synchronises the device and returns that word (0 =
+ * neither, bit 0: some wait gave up, bit 1: a page or a length was out of range, -1 = the
+ * word could not be read); `reset` != 0 clears it.
  * No counterpart in the reference.
  */
 int faws_device_status(int32_t reset);
