@@ -11,6 +11,7 @@ from .api import (  # noqa: F401
     attention_with_row_sum,
     attention_with_scores,
     attention_with_softmax_col_sum,
+    attention_with_window,
     compute_attention_scores,
     device_status,
     last_backend,
@@ -31,6 +32,7 @@ __all__ = [
     "attention_cross_token_qk_sum",
     "total_attention",
     "compute_attention_scores",
+    "attention_with_window",
     "KVCache4",
     "kv_cache_write",
     "kv_cache_read",

@@ -236,6 +236,62 @@ def attention(q, k, v, causal=False, sm_scale=None, dropout_p=0.0,
     return out
 
 
+_NO_LIMIT = 2 ** 31 - 1
+
+
+def _window_forward(q, k, v, window, sinks, sm_scale, need_L, backend, kv_splits):
+    c = _Call(q, k, v, True, sm_scale, 0.0, need_L=need_L, backend=backend)
+    n_splits = int(c.lib.faws_window_split_plan(C.byref(c.p), window, sinks)) if kv_splits is None else int(kv_splits)
+    ws, n = c.workspace(_lib.OP_ATTENTION_SPLIT_KV, n_splits) if n_splits > 1 else (None, 0)
+    c.run("faws_attention_with_window", window, sinks, n_splits, C.c_void_p(ws.data_ptr() if ws is not None else None), n)
+    return c
+
+
+class _WindowFunction(torch.autograd.Function):
+    """attention_with_window() under autograd, in the manner of _AttentionFunction."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, window, sinks, sm_scale, backend, kv_splits):
+        c = _window_forward(q, k, v, window, sinks, sm_scale, True, backend, kv_splits)
+        ctx.save_for_backward(c.q, c.k, c.v, c.out, c.L)
+        ctx.window, ctx.sinks, ctx.sm_scale, ctx.backend = window, sinks, float(c.p.sm_scale), backend
+        ctx.mark_non_differentiable(c.L)
+        ctx.set_materialize_grads(False)
+        return c.out, c.L
+
+    @staticmethod
+    def backward(ctx, do, *ignored):
+        q, k, v, o, L = ctx.saved_tensors
+        if do is None:
+            return (*map(torch.zeros_like, (q, k, v)), *(None,) * 5)
+        do = maybe_contiguous(do)
+        c = _Call(q, k, v, True, ctx.sm_scale, 0.0, out=o, L=L, backend=ctx.backend)
+        dq, dk, dv = torch.empty_like(c.q), torch.empty_like(c.k), torch.empty_like(c.v)
+        g = _lib.Grads(_tensor(do), _tensor(dq), _tensor(dk), _tensor(dv))
+        ws, n = c.workspace(_lib.OP_ATTENTION_BACKWARD)
+        c.run("faws_attention_with_window_backward", C.byref(g), ctx.window, ctx.sinks, C.c_void_p(ws.data_ptr()), n)
+        return dq, dk, dv, None, None, None, None, None
+
+
+def attention_with_window(q, k, v, window, sinks=0, sm_scale=None, return_log_normalizer=False,
+                          *, backend=None, kv_splits=None):
+    """Causal attention to a bounded context, differentiable in q, k, v: a query sees the last ``window`` keys up to its own
+    position (bottom-right aligned, as everywhere) and the first ``sinks`` keys of the sequence; rows that see none are zero.
+    Hidden keys and values must be finite, as in ``attention``: a weight of zero times an infinity is not zero.
+
+    Any number of rows, one included; with few of them the keys are cut into ranges as in ``attention``, and ``kv_splits`` pins
+    how many (1 = never).  Returns ``out``, or ``(out, log_normalizer)``.  No counterpart in the reference."""
+    window, sinks = min(int(window), _NO_LIMIT), min(int(sinks), _NO_LIMIT)
+    assert window >= 1, "window must be at least 1"
+    assert sinks >= 0, "sinks must not be negative"
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        out, L = _WindowFunction.apply(q, k, v, window, sinks, sm_scale, backend, kv_splits)
+    else:
+        c = _window_forward(q, k, v, window, sinks, sm_scale, return_log_normalizer, backend, kv_splits)
+        out, L = c.out, c.L
+    return (out, L) if return_log_normalizer else out
+
+
 def attention_with_scores(q, k, v, causal=False, sm_scale=None, dropout_p=0.0,
                           *, scores_dtype=torch.float32, masked_value=float("-inf"),
                           q_rows=None, backend=None, out=None, scores=None, philox=None):

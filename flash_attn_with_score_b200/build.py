@@ -26,8 +26,8 @@ LIB = os.path.join(HERE, "libfaws.so")
 PLAIN = os.path.join(HERE, "_plain.so")
 PLAIN_SOURCE = os.path.join(CSRC, "faws_torch.cpp")
 SOURCES = ["faws_abi.cu", "faws_generic.cu", "faws_tc.cu", "faws_tc_scores.cu", "faws_bwd.cu", "faws_tc_bwd.cu", "faws_noalloc.cu",
-           "faws_cache.cu"]
-HEADERS = ["faws_internal.cuh", "faws_tc_ptx.cuh", "faws_tc_host.cuh", "faws_tc_store.cuh", "faws_launch_plan.h"]
+           "faws_cache.cu", "faws_tc_window.cu"]
+HEADERS = ["faws_internal.cuh", "faws_tc_ptx.cuh", "faws_tc_host.cuh", "faws_tc_store.cuh", "faws_tc_fwd.cuh", "faws_launch_plan.h"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

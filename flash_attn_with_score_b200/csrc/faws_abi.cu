@@ -1,9 +1,11 @@
 // extern "C" entry points declared in include/faws.h: argument validation,
 // workspace carving, kernel-family selection and the launch sequences.
+#include <algorithm>
 #include <atomic>
 #include <cstdio>
 
 #include "faws_internal.cuh"
+#include "faws_launch_plan.h"
 #include "faws_tc_store.cuh"
 
 namespace faws {
@@ -301,10 +303,11 @@ struct SplitPlan {
 // wave.  Where launch_us expects more than 1.25 times the best count's time (inside that its own error could decide) the
 // best count is taken: bf16 D128 causal, B4 Hq16 Hk4 M200 N1500 17 us unsplit, 44 in six ranges; B2 H12 M500 N512 9.9 us
 // unsplit, 25.4 cut in four.
-SplitPlan plan_splits(const faws_problem* p, int sms) {
+// `nkt`: the key tiles to cut, all of them unless said.
+SplitPlan plan_splits(const faws_problem* p, int sms, int nkt = 0) {
   const long long ctas = (long long)p->B * p->Hq * cdiv(p->M, kTcBlockM);
   const long long rows = (long long)p->B * p->Hq * p->M;
-  const int nkt = cdiv(p->N, kTcBlockN);
+  if (nkt == 0) nkt = cdiv(p->N, kTcBlockN);
   const SplitPlan whole{1, launch_us(ctas, nkt, 1, p->D, rows, sms)};
   if (ctas * 10 >= 8LL * sms) return whole;
   int max_splits = sms < nkt ? sms : nkt;
@@ -441,6 +444,52 @@ bool forward_draws_mask(const faws_problem* p) {
   const long long heads = (long long)p->B * p->Hq, sms = device_sms();
   const long long tiles = heads * cdiv(p->M, 128), ctas = heads * cdiv(p->M, 256);
   return p->causal ? 2 * tiles >= 5 * sms : 6 * 2 * sms * ((ctas + sms - 1) / sms) <= 7 * tiles;
+}
+
+// Windows and sinks beyond any length are the same as 2^30, which leaves room to add positions.
+int clamp_span(int x) { return x > (1 << 30) ? 1 << 30 : x; }
+
+int validate_window(const faws_problem* p, int window, int sinks) {
+  const int st = validate(p);
+  if (st != FAWS_OK) return st;
+  if (window < 1 || sinks < 0 || !p->causal || p->m_begin != 0 || p->m_end != p->M) return FAWS_EINVAL;
+  if (p->M > (1 << 29) || p->N > (1 << 29)) return FAWS_EINVAL;
+  return p->dropout_p > 0.f ? FAWS_EUNSUPPORTED : FAWS_OK;
+}
+
+// The key tiles that a row block of a windowed problem visits at most (its list is cut into the split ranges).
+int window_list(const FwdParams& f) {
+  int most = 1;
+  if (f.pack_m > 0) return std::max(1, key_tiles(0, f.pack_m, f.p_seq, f.N, f.window, f.sinks).count());
+  const int blocks = cdiv(f.M, kTcBlockM);  // (lists grow along the rows until they are all alike, but for a last block cut short)
+  for (int r = std::max(0, blocks - 2) * kTcBlockM; r < f.M; r += kTcBlockM)
+    most = std::max(most, key_tiles(r, std::min(r + kTcBlockM, f.M), f.p_seq, f.N, f.window, f.sinks).count());
+  return most;
+}
+
+// The forward parameters of a windowed problem.  Few rows of grouped queries are packed as in use_packed (*p is replaced by the
+// packed problem then): where the packed rows fill no more tiles than one head's do.
+FwdParams make_fwd_window(const faws_problem** p, faws_problem* packed, int window, int sinks) {
+  const faws_problem* q = *p;
+  const int G = q->Hq / q->Hk;
+  int pack_m = 0;
+  if (tc_allowed(q) && G > 1 && (long long)G * q->M <= kTcBlockM && q->N >= q->M &&
+      q->q.stride_h == (int64_t)q->M * q->q.stride_s && q->out.stride_h == (int64_t)q->M * q->out.stride_s) {
+    *packed = *q;
+    packed->Hq = q->Hk;
+    packed->M = packed->m_end = G * q->M;
+    packed->q.stride_h = q->q.stride_h * G;
+    packed->out.stride_h = q->out.stride_h * G;
+    FwdParams f = make_fwd_packed(packed, q->M);
+    if (f.v != nullptr && tc_fwd_supported(f, packed->dtype)) {
+      pack_m = q->M;
+      *p = packed;
+    }
+  }
+  FwdParams f = make_fwd_packed(*p, pack_m);
+  f.window = clamp_span(window);
+  f.sinks = clamp_span(sinks);
+  return f;
 }
 
 // The 4-bit cache and the sequences of a call; `rows` rows of each.
@@ -661,7 +710,7 @@ int faws_total_attention(const faws_problem* p, float* total, void* stream) {
 }
 
 static int backward(const faws_problem* p, const faws_grads* g, const void* mask, void* workspace, size_t workspace_bytes,
-                    void* stream) {
+                    void* stream, int window = 0, int sinks = 0) {
   int st = validate(p);
   if (st != FAWS_OK) return st;
   if (g == nullptr || p->v.ptr == nullptr || p->out.ptr == nullptr || p->log_normalizer == nullptr ||
@@ -691,6 +740,7 @@ static int backward(const faws_problem* p, const faws_grads* g, const void* mask
   b.p_seq = p->N - p->M; b.causal = p->causal ? 1 : 0; b.sm_scale = p->sm_scale;
   b.drop = make_drop(p);
   b.mask = static_cast<const uint32_t*>(mask);
+  b.window = window; b.sinks = sinks;
   const size_t mask_bytes = p->dropout_p > 0.f ? tc_bwd_mask_bytes(p->B, p->Hq, p->M, p->N) : 0;
   b.mask_scratch = mask_bytes > 0 && workspace_bytes >= need + mask_bytes;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -725,6 +775,54 @@ int faws_attention_backward_masked(const faws_problem* p, const faws_grads* g, c
   // (tensors that have moved since to where only the CUDA-core kernels can read them: those draw the mask themselves)
   if (mask == nullptr || mask_bytes < mask_bytes_of(p) || misaligned_ws(mask)) return FAWS_EWORKSPACE;
   return backward(p, g, mask, workspace, workspace_bytes, stream);
+}
+
+int32_t faws_window_split_plan(const faws_problem* p, int32_t window, int32_t sinks) {
+  if (validate_window(p, window, sinks) != FAWS_OK || !tc_allowed(p)) return 1;
+  if (p->v.ptr == nullptr || p->out.ptr == nullptr) return 1;
+  faws_problem packed;
+  const FwdParams f = make_fwd_window(&p, &packed, window, sinks);
+  if (!tc_fwd_supported(f, p->dtype)) return 1;
+  return plan_splits(p, device_sms(), window_list(f)).splits;
+}
+
+int faws_attention_with_window(const faws_problem* p, int32_t window, int32_t sinks, int32_t n_splits, void* workspace,
+                               size_t workspace_bytes, void* stream) {
+  int st = validate_window(p, window, sinks);
+  if (st != FAWS_OK) return st;
+  if (n_splits < 1 || n_splits > cdiv(p->N, kTcBlockN) || (long long)p->B * n_splits > 65535) return FAWS_EINVAL;
+  if (p->out.ptr == nullptr || p->v.ptr == nullptr) return FAWS_EINVAL;
+  if (n_splits > 1 && (workspace == nullptr || workspace_bytes < split_kv_bytes(p, n_splits) || misaligned_ws(workspace)))
+    return FAWS_EWORKSPACE;
+  faws_problem packed;
+  const faws_problem* whole = p;
+  FwdParams f = make_fwd_window(&p, &packed, window, sinks);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (n_splits == 1) {
+    int bm, bn;
+    return run_fwd(p, f, s, &bm, &bn);
+  }
+  if (!tc_allowed(p) || !tc_fwd_supported(f, p->dtype)) return FAWS_EBACKEND;
+  float* L_part = static_cast<float*>(workspace);
+  float* o_part = reinterpret_cast<float*>(static_cast<char*>(workspace) +
+                                           align256((size_t)p->B * p->Hq * n_splits * p->M * 4));
+  f.o = o_part;  // (B, Hq, n_splits, M, D)
+  f.L = L_part;
+  f.n_splits = n_splits;
+  f.tiles_per_split = cdiv(window_list(f), n_splits);
+  if (launch_tc_fwd(f, p->dtype, s) != cudaSuccess) return FAWS_ECUDA;
+  if (launch_combine_splits(o_part, L_part, p->out.ptr, p->out.stride_b, p->out.stride_h, p->out.stride_s,
+                            whole->log_normalizer, p->B, p->Hq, p->M, p->D, n_splits, p->dtype, s) != cudaSuccess)
+    return FAWS_ECUDA;
+  t_last_backend = FAWS_BACKEND_TCGEN05;
+  return FAWS_OK;
+}
+
+int faws_attention_with_window_backward(const faws_problem* p, const faws_grads* g, int32_t window, int32_t sinks,
+                                        void* workspace, size_t workspace_bytes, void* stream) {
+  const int st = validate_window(p, window, sinks);
+  if (st != FAWS_OK) return st;
+  return backward(p, g, nullptr, workspace, workspace_bytes, stream, clamp_span(window), clamp_span(sinks));
 }
 
 size_t faws_workspace_bytes(int32_t op, const faws_problem* p, int32_t split) {

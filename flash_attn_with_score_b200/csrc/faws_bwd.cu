@@ -130,6 +130,7 @@ __global__ void __launch_bounds__(NT) generic_bwd_kv_kernel(BwdParams p) {
     const T* qp = reinterpret_cast<const T*>(p.q) + b * p.q_sb + h * p.q_sh;
     const T* gp = reinterpret_cast<const T*>(p.dout) + b * p.do_sb + h * p.do_sh;
     for (int m0 = (i_start / BT) * BT; m0 < p.M; m0 += BT) {
+      if (p.window > 0 && n0 + BT <= m0 + p.p_seq - p.window + 1 && n0 >= p.sinks) break;  // nor do later queries see a key
       __syncthreads();
       load_rows(Qs, lds, qp, p.q_ss, m0, p.M, D);
       load_rows(Gs, lds, gp, p.do_ss, m0, p.M, D);
@@ -148,7 +149,8 @@ __global__ void __launch_bounds__(NT) generic_bwd_kv_kernel(BwdParams p) {
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           const int j = n0 + tx + 16 * c;
-          const bool vis = i < p.M && j < p.N && (!p.causal || j <= i + p.p_seq);
+          const bool vis = i < p.M && j < p.N && (!p.causal || j <= i + p.p_seq) &&
+                         (p.window == 0 || j > i + p.p_seq - p.window || j < p.sinks);
           const PairGrad pg = pair_grad(p, s[r][c], dp[r][c], Ls[ty * 4 + r], Ds[ty * 4 + r], vis,
                                         ((uint32_t)bh * (uint32_t)p.M + (uint32_t)i) * (uint32_t)p.N + (uint32_t)j);
           Ps[(ty * 4 + r) * SLD + tx + 16 * c] = to_f(from_f<T>(pg.p_v));  // P is rounded like the forward pass rounds it
@@ -231,6 +233,7 @@ __global__ void __launch_bounds__(NT) generic_bwd_q_kernel(BwdParams p) {
   int hi = p.N;
   if (p.causal) hi = max(0, min(p.N, p.p_seq + min(m0 + BT, p.M)));
   for (int n0 = 0; n0 < hi; n0 += BT) {
+    if (p.window > 0 && n0 + BT <= m0 + p.p_seq - p.window + 1 && n0 >= p.sinks) continue;
     __syncthreads();
     load_rows(Ks, lds, kp, p.k_ss, n0, p.N, D);
     load_rows(Vs, lds, vp, p.v_ss, n0, p.N, D);
@@ -244,7 +247,8 @@ __global__ void __launch_bounds__(NT) generic_bwd_q_kernel(BwdParams p) {
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         const int j = n0 + tx + 16 * c;
-        const bool vis = i < p.M && j < p.N && (!p.causal || j <= i + p.p_seq);
+        const bool vis = i < p.M && j < p.N && (!p.causal || j <= i + p.p_seq) &&
+                         (p.window == 0 || j > i + p.p_seq - p.window || j < p.sinks);
         const PairGrad pg = pair_grad(p, s[r][c], dp[r][c], Ls[ty * 4 + r], Ds[ty * 4 + r], vis,
                                       ((uint32_t)bh * (uint32_t)p.M + (uint32_t)i) * (uint32_t)p.N + (uint32_t)j);
         dSs[(ty * 4 + r) * SLD + tx + 16 * c] = pg.ds;

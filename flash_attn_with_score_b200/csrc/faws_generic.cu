@@ -136,6 +136,7 @@ __global__ void __launch_bounds__(NT) generic_fwd_kernel(FwdParams p, int vec) {
     if (p.schedule == kReverse) t = nt - 1 - it;
     else if (p.schedule == kRoundRobin) t = (qb_abs + it) % nt;
     const int n0 = t * BN;
+    if (p.window > 0 && n0 + BN <= m0 + p.p_seq - p.window + 1 && n0 >= p.sinks) continue;  // nobody sees it
     __syncthreads();
     load_tile(Ks, lds, kp, p.k_ss, n0, 0, p.N, D, vec);
     load_tile(Vs, lds, vp, p.v_ss, n0, 0, p.N, D, vec);
@@ -151,7 +152,8 @@ __global__ void __launch_bounds__(NT) generic_fwd_kernel(FwdParams p, int vec) {
         const int j = n0 + tx + 16 * c;
         const float s = acc[r][c] * p.sm_scale;
         const bool inb = i >= p.m_begin && i < p.m_end && j < p.N;
-        const bool vis = inb && (!p.causal || j <= i + p.p_seq);
+        const bool vis = inb && (!p.causal || j <= i + p.p_seq) &&
+                         (p.window == 0 || j > i + p.p_seq - p.window || j < p.sinks);
         if (p.scores != nullptr && inb) {
           const int64_t off = (bh * p.M + i) * (int64_t)p.N + j;
           const float val = vis ? s : masked_f;

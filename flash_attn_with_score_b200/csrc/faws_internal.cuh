@@ -105,6 +105,7 @@ struct FwdParams {
   DropoutParams drop;
   uint32_t* drop_mask;   // tcgen05 attention(): the mask in memory (mask_word), or null
   int mask_drawn;        // launch_dropout_mask has drawn it; 0: the forward kernel draws it and leaves it there
+  int window, sinks;     // window > 0: a row sees its last `window` keys and the first `sinks` (causal is 1 then)
   int early_tiles;       // tcgen05 score launches: the first tiles fetched into L2 before the wait on the previous kernel
 };
 
@@ -188,6 +189,7 @@ struct BwdParams {
   DropoutParams drop;  // out_scale unused: the kept weights are rescaled by 1/(1-p) (flash.py:655,713,724)
   int mask_scratch;    // dropout, tcgen05: the workspace has room for the mask behind the rest
   const uint32_t* mask;  // dropout, tcgen05: the mask that the forward pass read, or null
+  int window, sinks;     // as in FwdParams
 };
 
 // Score-only operator (compute_attention_scores, attention_scores.py:154-223): scores = q.k^T * sm_scale.
@@ -259,6 +261,7 @@ cudaError_t launch_combine_splits(const float* o_part, const float* L_part, void
                                   cudaStream_t s);
 
 // tcgen05 family.  tc_supported() is a pure host-side check.
+cudaError_t launch_tc_fwd_window(const FwdParams& p, int dtype, cudaStream_t s);  // faws_tc_window.cu; called by launch_tc_fwd
 bool tc_fwd_supported(const FwdParams& p, int dtype);
 cudaError_t launch_tc_fwd(const FwdParams& p, int dtype, cudaStream_t s);
 bool tc_colsoftmax_supported(const ColSoftmaxParams& p, int dtype);

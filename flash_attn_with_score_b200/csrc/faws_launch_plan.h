@@ -13,6 +13,29 @@ namespace faws {
 
 constexpr int kPlanTile = 128;  // query rows and keys of a tile
 
+// The key tiles that query rows [first, end) visit when a row sees its last `window` keys and the first `sinks` (row i
+// stands at key i + p_seq): the `ns` tiles that hold sinks before the windows, then tiles [w0, end) of the windows.
+#ifdef __CUDACC__
+#define FAWS_HOST_DEVICE __host__ __device__ __forceinline__
+#else
+#define FAWS_HOST_DEVICE inline
+#endif
+struct KeyTiles {
+  int ns, w0, end;
+  FAWS_HOST_DEVICE int count() const { return ns + end - w0; }
+  FAWS_HOST_DEVICE int tile(int it) const { return it < ns ? it : w0 + it - ns; }
+};
+FAWS_HOST_DEVICE KeyTiles key_tiles(int first, int end, int p_seq, int N, int window, int sinks) {
+  int hi = p_seq + end;  // the keys before it are visible to the last row, if any
+  if (hi > N) hi = N;
+  if (hi <= 0 || end <= first) return {0, 0, 0};
+  int lo = p_seq + first - window + 1;
+  if (lo < 0) lo = 0;
+  int ns = ((sinks < N ? sinks : N) + kPlanTile - 1) / kPlanTile;
+  if (ns > lo / kPlanTile) ns = lo / kPlanTile;
+  return {ns, lo / kPlanTile, (hi + kPlanTile - 1) / kPlanTile};
+}
+
 // Persistent launches: one CTA per SM walks a list of work items (an item is what one CTA of the
 // plain launch does: a row block of one head), in the order of the plain launch's grid.  The
 // lists are made on the host (longest item first onto the least loaded CTA) and travel as a
@@ -31,6 +54,7 @@ struct WorkList {
 // The plain launch a list is made for.
 struct WorkShape {
   int gx, gy, gz, lpt, causal, p_seq, m_begin, m_end, N, rows, ctas, pack_m;
+  int window, sinks;  // window 0: none
   bool operator==(const WorkShape& o) const { return std::memcmp(this, &o, sizeof(WorkShape)) == 0; }
 };
 
@@ -48,6 +72,7 @@ inline std::vector<int> block_costs(const WorkShape& sh) {
         hi = sh.causal && sh.pack_m == 0 ? std::max(0, std::min(sh.N, sh.p_seq + std::min(r + kPlanTile, sh.m_end))) : sh.N;
       tiles = std::max(tiles, (hi + kPlanTile - 1) / kPlanTile);
     }
+    if (sh.window > 0) tiles = key_tiles(r0, std::min(r0 + sh.rows, sh.m_end), sh.p_seq, sh.N, sh.window, sh.sinks).count();
     cost[slot] = 19 * tiles + 30;  // measured on cfg3: 1.90 us per key tile + 3.0 us per item (unit 0.1 us)
   }
   return cost;
@@ -119,7 +144,7 @@ inline bool make_work_list(const WorkShape& sh, WorkList* out) {
   const int n_items = sh.gx * sh.gy * sh.gz, ctas = sh.ctas;
   if (ctas > kMaxListCtas || n_items <= ctas || n_items > 65535) return false;
   const bool listed = n_items <= kMaxListedItems;
-  if (!listed && sh.causal) return false;  // unequal items in no useful order: leave them to the hardware
+  if (!listed && sh.causal && sh.window == 0) return false;  // unequal items in no useful order: leave them to the hardware
   if (n_items < 2 * ctas) {
     *out = WorkList{n_items, 1, sh.gx, sh.gy, sh.gz, {}, {}};
     deal_short(sh, block_costs(sh), out);
@@ -218,6 +243,7 @@ inline bool make_work_list(const WorkShape& sh, WorkList* out) {
 struct RowChoice {
   long long heads;  // of all batches
   int m_begin, m_end, N, p_seq, causal, sms;
+  int window = 0, sinks = 0;  // window 0: none
   int blocks(int rows) const { return (m_end - m_begin + rows - 1) / rows; }
 };
 enum RowChoiceKind { kPlainOut, kWithRowSums, kWithColSums };
@@ -252,7 +278,8 @@ inline double expected_us(const RowChoice& c, bool d128, RowChoiceKind kind, int
   auto job = [&](int cb) -> double {
     const int end = std::min(c.m_begin + (cb + 1) * rows, c.m_end);
     const int hi = c.causal ? std::max(0, std::min(c.N, c.p_seq + end)) : c.N;
-    const int tiles = (hi + kPlanTile - 1) / kPlanTile;
+    int tiles = (hi + kPlanTile - 1) / kPlanTile;
+    if (c.window > 0) tiles = key_tiles(c.m_begin + cb * rows, end, c.p_seq, c.N, c.window, c.sinks).count();
     const bool ragged = cb == ncb - 1 && (c.m_end - c.m_begin) % kPlanTile != 0;
     return tiles == 0 ? f.empty : f.fix + (f.per + (ragged ? f.ragged : 0.0)) * tiles;
   };

@@ -45,6 +45,7 @@
 #include <type_traits>
 
 #include "faws_internal.cuh"
+#include "faws_launch_plan.h"
 #include "faws_tc_host.cuh"
 #include "faws_tc_ptx.cuh"
 
@@ -116,6 +117,7 @@ struct BwTcParams {
   int g_blocks, v_blocks;
   const uint32_t* mask;  // dropout: the mask as the pre-pass has drawn it (see draw_mask), or null
   int bh0;               // dropout: the launch's first (batch, head)
+  int window, sinks;     // WIN: a query sees its last `window` keys and the first `sinks`
 };
 
 // The dropout mask (mask_word) in scratch, where the forward pass kept none.  Both kernels need it, and a kernel with nothing else to
@@ -187,7 +189,7 @@ __device__ __forceinline__ GradScale grad_scale(const BwTcParams& p, int b, int 
   return {__int_as_float((127 + k) << 23), __int_as_float((127 - k) << 23)};
 }
 
-template <typename T, int D, bool KM, int MODE>
+template <typename T, int D, bool KM, int MODE, bool WIN = false>
 __global__ void __launch_bounds__(NTHREADS, 1)
 tc_bwd_kernel(const __grid_constant__ BwMaps maps, const BwTcParams p, int* __restrict__ status) {
   using L = BwSmem<D, KM>;
@@ -220,12 +222,24 @@ tc_bwd_kernel(const __grid_constant__ BwMaps maps, const BwTcParams p, int* __re
   int u0 = 0, nu;
   if (KM) {
     if (p.causal) u0 = max(0, own0 - p.p_seq) / BT;  // first query tile with a row that sees key own0
-    nu = max(0, (p.M + BT - 1) / BT - u0);
+    int m_end = p.M;
+    // the last query that sees a key of the tile is the one at the end of its last key's window; sinks are seen by all
+    if (WIN && own0 >= p.sinks) m_end = max(0, min(p.M, own0 + BT - 1 - p.p_seq + p.window));
+    nu = max(0, (m_end + BT - 1) / BT - u0);
   } else {
     int hi = p.N;
     if (p.causal) hi = max(0, min(p.N, p.p_seq + min(own0 + BT, p.M)));
     nu = (hi + BT - 1) / BT;
   }
+  [[maybe_unused]] KeyTiles kts{};
+  if constexpr (WIN && !KM) {
+    kts = key_tiles(own0, min(own0 + BT, p.M), p.p_seq, p.N, p.window, p.sinks);
+    nu = kts.count();
+  }
+  auto first_row = [&](int u) -> int {  // of streamed tile u
+    if constexpr (WIN && !KM) return kts.tile(u) * BT;
+    return (u0 + u) * BT;
+  };
 
   // Launch chain: pre-pass, query-major, key-major, group sum, each allowed to begin while the one before it drains.
   // Only the key-major kernel's partials and the pre-pass's arrays pass between them: the query-major kernel waits
@@ -286,7 +300,7 @@ tc_bwd_kernel(const __grid_constant__ BwMaps maps, const BwTcParams p, int* __re
       };
       load_tile(L::x_off, &maps.x, &bars->x_full, own0, x_head);
       for (int u = 0; u < nu; ++u) {
-        const int row0 = (u0 + u) * BT, sa = u % NA, sb = u % NB;
+        const int row0 = first_row(u), sa = u % NA, sb = u % NB;
         if (u >= NA && !mbar_wait(&bars->a_empty[sa], (u / NA - 1) & 1, abort_flag)) break;
         load_tile(L::a_off + sa * L::kTile, &maps.a, &bars->a_full[sa], row0, a_head);
         if (u == 0) load_tile(L::y_off, &maps.y, &bars->y_full, own0, x_head);
@@ -457,7 +471,7 @@ tc_bwd_kernel(const __grid_constant__ BwMaps maps, const BwTcParams p, int* __re
     // One streamed tile, kMasked where an entry of this warpgroup's 128 x 64 block may be hidden.
     auto tile_body = [&](auto masked_tag, int u) -> bool {
       constexpr bool kMasked = decltype(masked_tag)::value;
-      const int str0 = (u0 + u) * BT + e * HALF;  // first streamed row of this half
+      const int str0 = first_row(u) + e * HALF;  // first streamed row of this half
       // causal: (query i, key j) is visible iff j <= i + p_seq.  Column x of the half is streamed row
       // str0 + x.  Key-major (own = j, streamed = i): visible iff x >= own - p_seq - str0.
       // Query-major (own = i, streamed = j): visible iff x <= own + p_seq - str0.
@@ -470,6 +484,16 @@ tc_bwd_kernel(const __grid_constant__ BwMaps maps, const BwTcParams p, int* __re
         // 1 / (1 - p), which fp16 need not hold.
         if (KM && MODE == kDrop) x_hi = p.M - 1 - str0;
         if (!KM) x_hi = min(p.N - 1, p.causal ? own + p.p_seq : p.N - 1) - str0;
+      }
+      // Windows.  Key-major: visible while own >= i + p_seq - window + 1, or always, for a sink.  Query-major: the window's
+      // keys start at column x_lo, the sinks are those before column x_sink.
+      [[maybe_unused]] int x_sink = 0;
+      if constexpr (kMasked && WIN) {
+        if (KM && own >= p.sinks) x_hi = min(x_hi, own - p.p_seq + p.window - 1 - str0);
+        if (!KM) {
+          x_lo = own + p.p_seq - p.window + 1 - str0;
+          x_sink = p.sinks - str0;
+        }
       }
       [[maybe_unused]] uint32_t keep[2] = {~0u, ~0u};  // bit x of the pair: entry x of this thread's 64 is kept
       if (MODE == kDrop && p.mask != nullptr) {
@@ -525,7 +549,7 @@ tc_bwd_kernel(const __grid_constant__ BwMaps maps, const BwTcParams p, int* __re
 #pragma unroll
           for (int y = 0; y < 4; ++y) {
             float pe = fast_exp2(t[y]);
-            if (kMasked && !(x + y >= x_lo && x + y <= x_hi)) pe = 0.f;
+            if (kMasked && !(((x + y >= x_lo) || (WIN && !KM && x + y < x_sink)) && x + y <= x_hi)) pe = 0.f;
             sv[x + y] = __float_as_uint(pe);
             pr[y] = pe;
             // a product, not a select: a weight that is not finite stays visible where it is dropped
@@ -612,10 +636,14 @@ tc_bwd_kernel(const __grid_constant__ BwMaps maps, const BwTcParams p, int* __re
     };
     bool alive = true;
     for (int u = 0; alive && u < nu; ++u) {
-      const int str0 = (u0 + u) * BT + e * HALF;
+      const int str0 = first_row(u) + e * HALF;
       bool masked;
       if (KM) masked = (p.causal && own0 + BT - 1 - p.p_seq > str0) || (MODE == kDrop && str0 + HALF > p.M);
       else masked = str0 + HALF > (p.causal ? min(p.N, own0 + p.p_seq + 1) : p.N);
+      if constexpr (WIN) {
+        if (KM) masked = masked || (own0 + BT > p.sinks && str0 + HALF - 1 > max(own0, p.sinks) - p.p_seq + p.window - 1);
+        else masked = masked || (str0 + HALF > p.sinks && str0 < own0 + BT + p.p_seq - p.window);
+      }
       alive = masked ? tile_body(std::true_type{}, u) : tile_body(std::false_type{}, u);
     }
 
@@ -942,14 +970,14 @@ BwWs bwd_ws(int B, int Hq, int Hk, int M, int N, int D, bool fine) {
   return w;
 }
 
-template <typename T, int D, int MODE>
+template <typename T, int D, int MODE, bool WIN = false>
 cudaError_t launch_bwd_td(const BwdParams& p, cudaStream_t s) {
   using Lk = BwSmem<D, true>;
   using Lq = BwSmem<D, false>;
   static PerDeviceOnce once_km, once_qm;
   cudaError_t e;
-  if ((e = set_max_smem_once(once_km, tc_bwd_kernel<T, D, true, MODE>, Lk::total)) != cudaSuccess) return e;
-  if ((e = set_max_smem_once(once_qm, tc_bwd_kernel<T, D, false, MODE>, Lq::total)) != cudaSuccess) return e;
+  if ((e = set_max_smem_once(once_km, tc_bwd_kernel<T, D, true, MODE, WIN>, Lk::total)) != cudaSuccess) return e;
+  if ((e = set_max_smem_once(once_qm, tc_bwd_kernel<T, D, false, MODE, WIN>, Lq::total)) != cudaSuccess) return e;
   const int Mpad = mpad_of(p.M);
   const BwWs ws = bwd_ws(p.B, p.Hq, p.Hk, p.M, p.N, p.D, MODE != kPlain);
   char* base = reinterpret_cast<char*>(p.delta);
@@ -978,6 +1006,7 @@ cudaError_t launch_bwd_td(const BwdParams& p, cudaStream_t s) {
   tp.Hq = p.Hq; tp.G = p.G; tp.M = p.M; tp.N = p.N; tp.p_seq = p.p_seq; tp.causal = p.causal; tp.Mpad = Mpad;
   tp.sm_scale = p.sm_scale; tp.negl2 = negl2; tp.neg_delta = neg_delta; tp.D = p.D;
   tp.drop = p.drop;
+  tp.window = p.window; tp.sinks = p.sinks;
   tp.keep_scale = 1.f / (1.f - p.drop.p);
   tp.mask = p.mask != nullptr ? p.mask : mask;
   tp.g_stat = st.g; tp.v_stat = st.v; tp.g_blocks = st.g_blocks; tp.v_blocks = st.v_blocks;
@@ -1021,10 +1050,10 @@ cudaError_t launch_bwd_td(const BwdParams& p, cudaStream_t s) {
     tp.bh0 = tk.bh0 = bh0;
     const bool all = share == heads;
     const unsigned gx = all ? p.Hq : std::min(share, heads - bh0), gy = all ? p.B : 1;
-    if ((e = launch_overlapped(tc_bwd_kernel<T, D, false, MODE>, dim3(gx, gy, (p.M + BT - 1) / BT), NTHREADS, Lq::total, s,
+    if ((e = launch_overlapped(tc_bwd_kernel<T, D, false, MODE, WIN>, dim3(gx, gy, (p.M + BT - 1) / BT), NTHREADS, Lq::total, s,
                                qm, tp, status_word)) != cudaSuccess)
       return e;
-    if ((e = launch_overlapped(tc_bwd_kernel<T, D, true, MODE>, dim3(gx, gy, (p.N + BT - 1) / BT), NTHREADS, Lk::total, s,
+    if ((e = launch_overlapped(tc_bwd_kernel<T, D, true, MODE, WIN>, dim3(gx, gy, (p.N + BT - 1) / BT), NTHREADS, Lk::total, s,
                                km, tk, status_word)) != cudaSuccess)
       return e;
   }
@@ -1042,6 +1071,10 @@ cudaError_t launch_bwd_td(const BwdParams& p, cudaStream_t s) {
 
 template <typename T>
 cudaError_t launch_bwd_t(const BwdParams& p, cudaStream_t s) {
+  if (p.window > 0) {
+    if (p.D < 64) return launch_bwd_td<T, 64, kFine, true>(p, s);
+    return p.D == 128 ? launch_bwd_td<T, 128, kPlain, true>(p, s) : launch_bwd_td<T, 64, kPlain, true>(p, s);
+  }
   if (p.drop.p > 0.f) return p.D == 128 ? launch_bwd_td<T, 128, kDrop>(p, s) : launch_bwd_td<T, 64, kDrop>(p, s);
   if (p.D < 64) return launch_bwd_td<T, 64, kFine>(p, s);
   return p.D == 128 ? launch_bwd_td<T, 128, kPlain>(p, s) : launch_bwd_td<T, 64, kPlain>(p, s);

@@ -1,0 +1,28 @@
+// The forward launches of attention_with_window(): the forward kernel's instances whose rows see their last keys and the
+// first ones only.
+#include <cuda.h>
+
+#include "faws_tc_fwd.cuh"
+
+namespace faws {
+namespace {
+
+template <typename T, int D>
+cudaError_t launch_t(const TcMaps& maps, const FwdParams& p, cudaStream_t s) {
+  if (p.pack_m > 0 || p.n_splits > 1) return launch_fwd_s<T, D, kHookNone, true, kNoDrop, true, true>(maps, p, s);
+  const RowChoice c{(long long)p.B * p.Hq, p.m_begin, p.m_end, p.N, p.p_seq, p.causal, sm_count(), p.window, p.sinks};
+  const bool large = c.blocks(256) * c.heads >= 2LL * c.sms || prefer_256_rows(c, D == 128, kPlainOut);
+  return large ? launch_fwd_s<T, D, kHookNone, false, kNoDrop, false, true>(maps, p, s)
+               : launch_fwd_s<T, D, kHookNone, true, kNoDrop, false, true>(maps, p, s);
+}
+
+}  // namespace
+
+cudaError_t launch_tc_fwd_window(const FwdParams& p, int dtype, cudaStream_t s) {
+  TcMaps maps;
+  if (!make_fwd_maps(&maps, p)) return cudaErrorInvalidValue;
+  if (dtype == FAWS_FP16) return p.D == 128 ? launch_t<__half, 128>(maps, p, s) : launch_t<__half, 64>(maps, p, s);
+  return p.D == 128 ? launch_t<__nv_bfloat16, 128>(maps, p, s) : launch_t<__nv_bfloat16, 64>(maps, p, s);
+}
+
+}  // namespace faws

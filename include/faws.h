@@ -299,6 +299,24 @@ int faws_attention_backward_masked(const faws_problem* p, const faws_grads* g, c
 size_t faws_workspace_bytes(int32_t op, const faws_problem* p, int32_t split);
 
 /*
+ * Causal attention to a bounded context: query i, which stands at position i + N - M, sees the keys j <= i + N - M that are among
+ * its last `window` (j > i + N - M - window) or among the first `sinks` of the sequence (j < sinks).  window >= 1 (its own key is
+ * the first of them), sinks >= 0, p->causal 1, no dropout, no query-row window.  Key tiles that nobody sees are not
+ * read.  Otherwise as faws_attention, which it equals where window >= N.  No counterpart in the reference.
+ *
+ * n_splits: 1, or more for problems with few query rows, as faws_attention_split_kv takes them: the key tiles that a row block
+ * visits are cut into so many ranges.  faws_window_split_plan says how many the library would choose.
+ * Workspace for n_splits > 1: faws_workspace_bytes(FAWS_OP_ATTENTION_SPLIT_KV, p, n_splits).
+ *
+ * Backward pass: as faws_attention_backward, with its workspace.  Keys that no query sees get zero gradients.
+ */
+int32_t faws_window_split_plan(const faws_problem* p, int32_t window, int32_t sinks);
+int faws_attention_with_window(const faws_problem* p, int32_t window, int32_t sinks, int32_t n_splits, void* workspace,
+                               size_t workspace_bytes, void* stream);
+int faws_attention_with_window_backward(const faws_problem* p, const faws_grads* g, int32_t window, int32_t sinks,
+                                        void* workspace, size_t workspace_bytes, void* stream);
+
+/*
  * A paged cache of keys and values in 4 bits, and the operators on it.  No counterpart in the reference.
  *
  * A row (one token of one kv head) is cut into groups of min(32, D) neighbouring elements.  A group has a scale s =
