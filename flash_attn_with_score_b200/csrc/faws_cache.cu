@@ -47,8 +47,41 @@ template <> __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) 
   const __half2 h = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
+template <typename T> __device__ __forceinline__ float2 unpack2(uint32_t w);
+template <> __device__ __forceinline__ float2 unpack2<__half>(uint32_t w) { return __half22float2(*reinterpret_cast<__half2*>(&w)); }
+template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t w) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+__device__ __forceinline__ float fast_rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// (nibble - 8) * scale of both halves, rounded once; `scale` a bf16 number
+template <typename T> __device__ __forceinline__ uint32_t code_times_scale(uint32_t nibbles, uint32_t scale);
+template <> __device__ __forceinline__ uint32_t code_times_scale<__half>(uint32_t nibbles, uint32_t scale) {
+  nibbles |= 0x64006400u;  // 1024 + n
+  const __half2 c = __hsub2(*reinterpret_cast<__half2*>(&nibbles), __floats2half2_rn(1032.f, 1032.f));
+  const float2 f = __half22float2(c);
+  const float s = __uint_as_float(scale << 16);  // (may be smaller than fp16 holds exactly)
+  const __half2 v = __floats2half2_rn(f.x * s, f.y * s);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <> __device__ __forceinline__ uint32_t code_times_scale<__nv_bfloat16>(uint32_t nibbles, uint32_t scale) {
+  nibbles |= 0x43004300u;  // 128 + n
+  scale |= scale << 16;
+  const __nv_bfloat162 c = __hsub2(*reinterpret_cast<__nv_bfloat162*>(&nibbles), __floats2bfloat162_rn(136.f, 136.f));
+  const __nv_bfloat162 v = __hmul2(c, *reinterpret_cast<__nv_bfloat162*>(&scale));
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
 __device__ __forceinline__ float bf16_lo(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float bf16_hi(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+
+__device__ __forceinline__ float fast_log2(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 
 // Length of sequence b as the cache can hold it; *bad where lengths says otherwise.
 __device__ __forceinline__ int cached_length(const CacheBatch& c, int page_shift, int b, bool* bad) {
@@ -60,118 +93,125 @@ __device__ __forceinline__ int cached_length(const CacheBatch& c, int page_shift
 }
 
 // ---------------------------------------------------------------------------------------------- write, read
-// A thread has 8 neighbouring elements of a row; D / 8 threads a row, the four (D 16: two) of a group next to each other.
-// Bound by HBM: 2 bytes read and 9/16 written an element (read: the other way round).
+// A thread has 8 neighbouring elements of a row; TPR = D / 8 threads a row, the four (D 16: two) of a group next to each other.
+// Bound by HBM: 2 bytes read and 9/16 written an element (reading back: the other way round).  A CTA takes consecutive rows
+// of one sequence and head, a thread kRowsEach of them, so that what a row costs beside its elements is little.
 struct CacheRows {
   const void* src[2];  // write: k, v; read: unused
   void* dst[2];        // read: k, v
   int64_t sb[2], sh[2], ss[2];
   int rows;            // of each sequence
+  int tiles;           // CTAs that the rows of a sequence and head take
   int vec;             // 16-byte accesses to them
 };
+constexpr int kRowsEach = 4;
 
-template <typename T>
-__device__ __forceinline__ void load8(float (&x)[8], const T* p, bool vec) {
-  if (vec) {
-    const uint4 w4 = *reinterpret_cast<const uint4*>(p);
-    const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
-#pragma unroll
-    for (int y = 0; y < 4; ++y) {
-      T e[2];
-      *reinterpret_cast<uint32_t*>(e) = w[y];
-      x[2 * y] = to_f(e[0]);
-      x[2 * y + 1] = to_f(e[1]);
-    }
-  } else {
-#pragma unroll
-    for (int y = 0; y < 8; ++y) x[y] = to_f(p[y]);
-  }
-}
-
-// the row's place: sequence, head, position; false where there is none (padding, or a page that does not exist)
-struct Place {
-  int b, hk, m, page;
-  int64_t token;  // row index into the cache's tensors
-};
-__device__ __forceinline__ bool find_place(const CacheParams& c, const CacheBatch& bt, int rows, int64_t row, Place* at,
-                                           bool* bad) {
-  at->m = (int)(row % rows);
-  const int64_t bh = row / rows;
-  at->hk = (int)(bh % c.Hk);
-  at->b = (int)(bh / c.Hk);
-  const int len = cached_length(bt, c.page_shift, at->b, bad);
-  const int pos = len - rows + at->m;
-  at->token = -1;
-  if (pos < 0) return false;
-  at->page = bt.table[(int64_t)at->b * bt.table_stride + (pos >> c.page_shift)];
-  if ((unsigned)at->page >= (unsigned)c.pages) {
+// Row of the cache's tensors that holds position pos; -1 for a page that does not exist.
+__device__ __forceinline__ int64_t cache_row(const CacheParams& c, const int32_t* table, int hk, int pos, bool* bad) {
+  const int page = table[pos >> c.page_shift];
+  if ((unsigned)page >= (unsigned)c.pages) {
     *bad = true;
-    return true;
+    return -1;
   }
-  at->token = (((int64_t)at->page * c.Hk + at->hk) << c.page_shift) + (pos & ((1 << c.page_shift) - 1));
-  return true;
+  return (((int64_t)page * c.Hk + hk) << c.page_shift) + (pos & ((1 << c.page_shift) - 1));
 }
+
+// The words of a row of values as they lie in memory, from the words of elements (`to` true), or back.  Word p of the row: half-words
+// g NG + gi of 2 p and 2 p + 1; the word of elements w = 4 gi + t: half-words of g = 2 t and 2 t + 1, group gi.
+template <int D>
+__device__ __forceinline__ uint32_t exchange_halves(uint32_t word, int w, bool to) {
+  if constexpr (D < 64) return word;  // one group: the same order
+  else {
+  constexpr int NG = D / 32, TPR = D / 8;
+  const int lane0 = (threadIdx.x & 31) & ~(TPR - 1);
+  // to memory: position w is g = 2 w / NG, groups gi and gi + 1, from the words 4 gi + g / 2 and 4 (gi + 1) + g / 2, half g & 1
+  // from memory: word 4 gi + t takes half-words (2 t) NG + gi and (2 t + 1) NG + gi: words t NG + gi / 2 and + NG / 2, half gi & 1
+  const int g = 2 * w / NG, gi = to ? 2 * w % NG : w / 4, t = w % 4;
+  const int from0 = to ? 4 * gi + g / 2 : t * NG + gi / 2;
+  const uint32_t a = __shfl_sync(0xffffffffu, word, lane0 + from0);
+  const uint32_t b = __shfl_sync(0xffffffffu, word, lane0 + from0 + (to ? 4 : NG / 2));
+  return __byte_perm(a, b, ((to ? g : gi) & 1) ? 0x7632 : 0x5410);
+  }
+}
+// each half rotated left by 2, and right
+__device__ __forceinline__ uint32_t rotate_halves(uint32_t x) { return (x << 2 & 0xfffcfffcu) | (x >> 14 & 0x00030003u); }
+__device__ __forceinline__ uint32_t rotate_halves_back(uint32_t x) { return (x >> 2 & 0x3fff3fffu) | (x << 14 & 0xc000c000u); }
 
 template <typename T, int D>
 __global__ void __launch_bounds__(256) cache_write_kernel(CacheParams c, CacheBatch bt, CacheRows r, int* status) {
   constexpr int TPR = D / 8, NG = D >= 32 ? D / 32 : 1, GL = D >= 32 ? 4 : 2;
+  constexpr uint32_t kInfinity = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
   griddep_wait();
   griddep_launch_dependents();
-  const int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int w = (int)(idx % TPR);
-  const int64_t row = idx / TPR;
+  const int w = threadIdx.x % TPR, lanes = blockDim.x / TPR;
+  const int bh = blockIdx.x / (unsigned)r.tiles, tile = blockIdx.x - bh * r.tiles;
+  const int b = bh / (unsigned)c.Hk, hk = bh - b * c.Hk;
   const bool second = blockIdx.y != 0;
-  const bool in = row < (int64_t)bt.B * c.Hk * r.rows;
-  Place at;
   bool bad = false;
-  const bool here = in && find_place(c, bt, r.rows, row, &at, &bad) && at.token >= 0;
-  float x[8];
+  const int first = cached_length(bt, c.page_shift, b, &bad) - r.rows;  // position of row 0
+  const int32_t* table = bt.table + (int64_t)b * bt.table_stride;
+  const T* src = static_cast<const T*>(second ? r.src[1] : r.src[0]) + b * (second ? r.sb[1] : r.sb[0]) +
+                 hk * (second ? r.sh[1] : r.sh[0]) + w * 8;
+  const int64_t ss = second ? r.ss[1] : r.ss[0];
+  unsigned char* codes = static_cast<unsigned char*>(second ? c.v_codes : c.k_codes);
+  uint16_t* scales = static_cast<uint16_t*>(second ? c.v_scales : c.k_scales);
+  const int m0 = tile * lanes * kRowsEach + threadIdx.x / TPR;
+  uint4 in[kRowsEach];
 #pragma unroll
-  for (int y = 0; y < 8; ++y) x[y] = 0.f;
-  if (here)
-    load8<T>(x, static_cast<const T*>(second ? r.src[1] : r.src[0]) + at.b * (second ? r.sb[1] : r.sb[0]) +
-                    at.hk * (second ? r.sh[1] : r.sh[0]) + (int64_t)at.m * (second ? r.ss[1] : r.ss[0]) + w * 8,
-             r.vec != 0);
-  // largest magnitude of the group; as integers the magnitudes order as they do, and infinities and NaN come last
-  uint32_t top = 0u;
+  for (int y = 0; y < kRowsEach; ++y) {
+    const int m = m0 + y * lanes;
+    in[y] = make_uint4(0u, 0u, 0u, 0u);
+    if (m < r.rows && first + m >= 0) {
+      if (r.vec) in[y] = *reinterpret_cast<const uint4*>(src + m * ss);
+      else {
+        uint16_t e[8];
 #pragma unroll
-  for (int y = 0; y < 8; ++y) top = max(top, __float_as_uint(x[y]) & 0x7fffffffu);
-#pragma unroll
-  for (int s = 1; s < GL; s <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, s));
-  uint32_t sbits;  // bf16
-  float inv = 0.f;
-  if (top >= 0x7f800000u) sbits = 0xffc0u;
-  else {
-    const __nv_bfloat16 s = __float2bfloat16_rn(__fdiv_rn(__uint_as_float(top), 7.f));
-    sbits = *reinterpret_cast<const uint16_t*>(&s);
-    if (sbits < 0x0080u) sbits = 0u;  // below the smallest normal number
-    else inv = __fdiv_rn(1.f + 9.5367431640625e-7f, __uint_as_float(sbits << 16));
-  }
-  uint32_t word = 0u;
-#pragma unroll
-  for (int y = 0; y < 8; ++y) {
-    const int mag = inv == 0.f ? 0 : (int)fmaf(fabsf(x[y]), inv, 0.5f);
-    word |= (uint32_t)(8 + (x[y] < 0.f ? -mag : mag)) << (4 * y);
-  }
-  if (here) {
-    if (!second) {
-      unsigned char* codes = static_cast<unsigned char*>(c.k_codes) + at.token * (D / 2);
-      const int gi = w / 4, t = w % 4;
-      if (D >= 32) *reinterpret_cast<uint32_t*>(codes + (t * NG + gi) * 4) = __funnelshift_l(word, word, 2);
-      else *reinterpret_cast<uint32_t*>(codes + w * 4) = word;  // half-word t: elements 4 t .. 4 t + 3
-    } else {
-      unsigned char* codes = static_cast<unsigned char*>(c.v_codes) + at.token * (D / 2);
-      const int gi = w / 4, t = w % 4;
-      if (D >= 32) {
-        word = (word << 2 & 0xfffcfffcu) | (word >> 14 & 0x00030003u);  // each half by itself
-        *reinterpret_cast<uint16_t*>(codes + (2 * t * NG + gi) * 2) = (uint16_t)word;
-        *reinterpret_cast<uint16_t*>(codes + ((2 * t + 1) * NG + gi) * 2) = (uint16_t)(word >> 16);
-      } else {
-        *reinterpret_cast<uint32_t*>(codes + w * 4) = word;  // byte g: elements 2 g, 2 g + 1
+        for (int x = 0; x < 8; ++x) e[x] = reinterpret_cast<const uint16_t*>(src + m * ss)[x];
+        in[y] = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
       }
     }
-    if (w % GL == 0)
-      static_cast<uint16_t*>(second ? c.v_scales : c.k_scales)[at.token * NG + w / GL] = (uint16_t)sbits;
+  }
+#pragma unroll
+  for (int y = 0; y < kRowsEach; ++y) {
+    const int m = m0 + y * lanes;
+    const uint32_t v[4] = {in[y].x, in[y].y, in[y].z, in[y].w};
+    // largest magnitude of the group, as integers, as which they order alike; infinities and NaN come last
+    uint32_t top = __vmaxu2(__vmaxu2(v[0] & 0x7fff7fffu, v[1] & 0x7fff7fffu), __vmaxu2(v[2] & 0x7fff7fffu, v[3] & 0x7fff7fffu));
+    top = max(top & 0xffffu, top >> 16);
+#pragma unroll
+    for (int s = 1; s < GL; s <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, s));
+    float x[8];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float2 f = unpack2<T>(v[e]);
+      x[2 * e] = f.x;
+      x[2 * e + 1] = f.y;
+    }
+    // (a product with the nearest number to 1/7, 2^-26 of it away, rounds to bf16 as the quotient does: amax has 11 bits at most, so
+    // amax / 7 is a number of 9 bits, which the product rounds to, or 2^-12 of itself from the middle of two bf16 numbers)
+    const __nv_bfloat16 s16 = __float2bfloat16_rn(unpack2<T>(top).x * (1.f / 7.f));
+    uint32_t sbits = *reinterpret_cast<const uint16_t*>(&s16);
+    if (sbits < 0x0080u) sbits = 0u;  // below the smallest normal number
+    // Codes c + 8 by one fma each, in the low bits of a sum with 2^23: with the quotients moved by 2^-20 of themselves there is
+    // no half to be rounded, and the nearest number is the definition's.  (s 0: the quotients are 0.)
+    float inv = sbits != 0u ? fast_rcp(__uint_as_float(sbits << 16)) * (1.f + 9.5367431640625e-7f) : 0.f;
+    if (top >= kInfinity) {
+      sbits = 0xffc0u;
+      inv = 0.f;
+    }
+    uint32_t word = __float_as_uint(fmaf(x[7], inv, 8388616.f));
+#pragma unroll
+    for (int e = 6; e >= 0; --e) word = word * 16u + __float_as_uint(fmaf(x[e], inv, 8388616.f));
+    word -= 0xfb000000u;  // what is left of 2^23, 0x4b000000 in elements 0 and 1
+    if (D >= 32) word = second ? exchange_halves<D>(rotate_halves(word), w, true) : __funnelshift_l(word, word, 2);
+    if (m < r.rows && first + m >= 0) {
+      const int64_t row = cache_row(c, table, hk, first + m, &bad);
+      if (row >= 0) {
+        const int at = D >= 32 && !second ? (w % 4) * NG + w / 4 : w;
+        *reinterpret_cast<uint32_t*>(codes + row * (D / 2) + at * 4) = word;
+        if (w % GL == 0) scales[row * NG + w / GL] = (uint16_t)sbits;
+      }
+    }
   }
   if (bad && status != nullptr) atomicOr(status, kBadPage);
 }
@@ -181,43 +221,54 @@ __global__ void __launch_bounds__(256) cache_read_kernel(CacheParams c, CacheBat
   constexpr int TPR = D / 8, NG = D >= 32 ? D / 32 : 1, GL = D >= 32 ? 4 : 2;
   griddep_wait();
   griddep_launch_dependents();
-  const int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int w = (int)(idx % TPR);
-  const int64_t row = idx / TPR;
-  if (row >= (int64_t)bt.B * c.Hk * r.rows) return;
+  const int w = threadIdx.x % TPR, lanes = blockDim.x / TPR;
+  const int bh = blockIdx.x / (unsigned)r.tiles, tile = blockIdx.x - bh * r.tiles;
+  const int b = bh / (unsigned)c.Hk, hk = bh - b * c.Hk;
   const bool second = blockIdx.y != 0;
-  Place at;
   bool bad = false;
-  const bool real = find_place(c, bt, r.rows, row, &at, &bad);
-  uint32_t word = 0x88888888u, sbits = 0u;  // padding: zeros
-  if (real && at.token < 0) sbits = 0xffc0u;
-  else if (real) {
-    sbits = static_cast<const uint16_t*>(second ? c.v_scales : c.k_scales)[at.token * NG + w / GL];
-    const int gi = w / 4, t = w % 4;
-    if (!second) {
-      const unsigned char* codes = static_cast<const unsigned char*>(c.k_codes) + at.token * (D / 2);
-      word = *reinterpret_cast<const uint32_t*>(codes + (D >= 32 ? (t * NG + gi) * 4 : w * 4));
-      if (D >= 32) word = __funnelshift_r(word, word, 2);
-    } else {
-      const unsigned char* codes = static_cast<const unsigned char*>(c.v_codes) + at.token * (D / 2);
-      if (D >= 32) {
-        word = (uint32_t)*reinterpret_cast<const uint16_t*>(codes + (2 * t * NG + gi) * 2) |
-               (uint32_t)*reinterpret_cast<const uint16_t*>(codes + ((2 * t + 1) * NG + gi) * 2) << 16;
-        word = (word >> 2 & 0x3fff3fffu) | (word << 14 & 0xc000c000u);
-      } else word = *reinterpret_cast<const uint32_t*>(codes + w * 4);
+  const int first = cached_length(bt, c.page_shift, b, &bad) - r.rows;
+  const int32_t* table = bt.table + (int64_t)b * bt.table_stride;
+  const unsigned char* codes = static_cast<const unsigned char*>(second ? c.v_codes : c.k_codes);
+  const uint16_t* scales = static_cast<const uint16_t*>(second ? c.v_scales : c.k_scales);
+  const int m0 = tile * lanes * kRowsEach + threadIdx.x / TPR;
+  const int at = D >= 32 && !second ? (w % 4) * NG + w / 4 : w;
+  uint32_t words[kRowsEach], sbits[kRowsEach];
+#pragma unroll
+  for (int y = 0; y < kRowsEach; ++y) {
+    const int m = m0 + y * lanes;
+    words[y] = D >= 32 ? 0x22222222u : 0x88888888u;  // padding: zeros
+    sbits[y] = 0u;
+    if (m < r.rows && first + m >= 0) {
+      const int64_t row = cache_row(c, table, hk, first + m, &bad);
+      sbits[y] = 0xffc0u;
+      if (row >= 0) {
+        words[y] = *reinterpret_cast<const uint32_t*>(codes + row * (D / 2) + at * 4);
+        sbits[y] = scales[row * NG + w / GL];
+      }
     }
   }
-  const float s = __uint_as_float(sbits << 16);
-  T* dst = static_cast<T*>(second ? r.dst[1] : r.dst[0]) + at.b * (second ? r.sb[1] : r.sb[0]) +
-           at.hk * (second ? r.sh[1] : r.sh[0]) + (int64_t)at.m * (second ? r.ss[1] : r.ss[0]) + w * 8;
-  uint32_t out[4];
+  T* dst = static_cast<T*>(second ? r.dst[1] : r.dst[0]) + b * (second ? r.sb[1] : r.sb[0]) +
+           hk * (second ? r.sh[1] : r.sh[0]) + w * 8;
+  const int64_t ss = second ? r.ss[1] : r.ss[0];
 #pragma unroll
-  for (int y = 0; y < 4; ++y)
-    out[y] = pack2<T>(s * (float)((int)(word >> (8 * y) & 15u) - 8), s * (float)((int)(word >> (8 * y + 4) & 15u) - 8));
-  if (r.vec) *reinterpret_cast<uint4*>(dst) = make_uint4(out[0], out[1], out[2], out[3]);
-  else {
+  for (int y = 0; y < kRowsEach; ++y) {
+    const int m = m0 + y * lanes;
+    uint32_t word = words[y];
+    if (D >= 32) word = second ? rotate_halves_back(exchange_halves<D>(word, w, false)) : __funnelshift_r(word, word, 2);
+    // elements (0, 4), (1, 5), (2, 6), (3, 7), each exact as a 16-bit number; their products are rounded once
+    uint32_t pair[4];
 #pragma unroll
-    for (int y = 0; y < 8; ++y) reinterpret_cast<uint16_t*>(dst)[y] = (uint16_t)(out[y / 2] >> (16 * (y & 1)));
+    for (int e = 0; e < 4; ++e) pair[e] = code_times_scale<T>(word >> (4 * e) & 0x000f000fu, sbits[y]);
+    const uint4 out = make_uint4(__byte_perm(pair[0], pair[1], 0x5410), __byte_perm(pair[2], pair[3], 0x5410),
+                                 __byte_perm(pair[0], pair[1], 0x7632), __byte_perm(pair[2], pair[3], 0x7632));
+    if (m < r.rows) {
+      if (r.vec) *reinterpret_cast<uint4*>(dst + m * ss) = out;
+      else {
+        const uint32_t o[4] = {out.x, out.y, out.z, out.w};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) reinterpret_cast<uint16_t*>(dst + m * ss)[e] = (uint16_t)(o[e / 2] >> (16 * (e & 1)));
+      }
+    }
   }
   if (bad && status != nullptr) atomicOr(status, kBadPage);
 }
@@ -243,16 +294,29 @@ __global__ void __launch_bounds__(256) cache_read_kernel(CacheParams c, CacheBat
 // Weights are fp16: 2^-12 of each.  The running maximum is that of S + log2 s, so that P s stays within fp16 for values of
 // any size; what falls below 2^-24 of the largest weighted value is lost.
 constexpr int TT = 128;       // tokens of a tile
-constexpr int STAGES = 4;
+constexpr int STAGES = 3;
 constexpr int CONSUMERS = 4;  // warps
 constexpr int CTA_THREADS = 32 * (CONSUMERS + 1);
-constexpr int CTAS_PER_SM = 2;
+__host__ __device__ constexpr int ctas_per_sm(int rt) { return rt == 8 ? 3 : 2; }
 constexpr uint32_t kLow = 0x003c003cu, kHigh = 0x03c003c0u;  // the two nibbles of each half's mantissa
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Without an accumulator to begin with.
+__device__ __forceinline__ void mma_f16_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+               : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+// 8 x 8 halves across a warp: on entry lane 4 i + j has elements (i, 2 j) and (i, 2 j + 1), on exit (2 j, i) and (2 j + 1, i).
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
 }
 
 // Barrier of the consumer warps; whether any thread said so.
@@ -372,6 +436,8 @@ struct CacheSmem {
   static constexpr int kOutRow = D + 4;
   static constexpr int ml_off = out_off + CONSUMERS * RT * kOutRow * 4;
   static constexpr int bar_off = ml_off + CONSUMERS * RT * 8;
+  // While a segment lasts a warp's part of the output area holds its 32 tokens' scales of keys and values as pairs of floats.
+  static_assert(2 * 32 * NG * 8 <= RT * kOutRow * 4, "room for the scales");
   static constexpr int total = bar_off + 128;
 };
 struct CacheBars {
@@ -405,7 +471,7 @@ __device__ __forceinline__ void store_row(const CacheAttnParams& p, int b, int h
 }
 
 template <typename T, int D, int RT>
-__global__ void __launch_bounds__(CTA_THREADS, CTAS_PER_SM) cache_attn_kernel(const CacheAttnParams p) {
+__global__ void __launch_bounds__(CTA_THREADS, ctas_per_sm(RT)) cache_attn_kernel(const CacheAttnParams p) {
   using L = CacheSmem<D, RT>;
   constexpr int NG = L::NG;
   constexpr int MT = D >= 32 ? 2 : 1;  // 16-row tiles of a group's output
@@ -442,36 +508,48 @@ __global__ void __launch_bounds__(CTA_THREADS, CTAS_PER_SM) cache_attn_kernel(co
                                                                  : kind == 1 ? p.cache.v_codes
                                                                  : kind == 2 ? p.cache.k_scales
                                                                              : p.cache.v_scales);
+    // what of tile `it` of the segment this lane copies, and the page that has it
+    struct Piece {
+      int t0, lo, hi, page;
+    };
+    auto piece_of = [&](int it) -> Piece {
+      Piece c;
+      c.t0 = w.span.tile(w.first + it) * TT;
+      // what may be seen of the tile: the sinks, the windows, or both
+      c.lo = max(c.t0, w.span.lo);
+      c.hi = min(c.t0 + TT, w.span.len);
+      if (c.t0 < p.sinks) {
+        if (c.lo >= c.hi) c.hi = min(c.hi, p.sinks);
+        c.lo = c.t0;
+      }
+      const int p0 = c.t0 + (piece << shift);
+      c.lo = max(c.lo, p0) & ~15;
+      c.hi = min((min(c.hi, p0 + (1 << shift)) + 15) & ~15, p0 + (1 << shift));
+      c.page = -1;
+      if (!mine) c.hi = c.lo;
+      if (c.lo < c.hi) c.page = p.batch.table[(int64_t)w.b * p.batch.table_stride + (p0 >> p.cache.page_shift)];
+      return c;
+    };
     int n = 0;  // tiles so far
     bool ok = true, bad = false;
     do {
       const int hk = w.item / p.row_blocks, cnt = w.count();
+      Piece next = piece_of(0);
       for (int it = 0; ok && it < cnt; ++it, ++n) {
-        const int t0 = w.span.tile(w.first + it) * TT;
-        // what may be seen of the tile: the sinks, the windows, or both
-        int lo = max(t0, w.span.lo), hi = min(t0 + TT, w.span.len);
-        if (t0 < p.sinks) {
-          if (lo >= hi) hi = min(hi, p.sinks);
-          lo = t0;
-        }
-        const int p0 = t0 + (piece << shift);
-        lo = max(lo, p0) & ~15;
-        hi = min((min(hi, p0 + (1 << shift)) + 15) & ~15, p0 + (1 << shift));
+        const Piece c = next;
+        if (it + 1 < cnt) next = piece_of(it + 1);  // (its page comes while the tile before it waits for room)
         const int s = n % STAGES;
-        unsigned char* stage = smem + s * L::kStage;
-        int page = -1;
-        const bool copy = mine && lo < hi;
-        if (copy) page = p.batch.table[(int64_t)w.b * p.batch.table_stride + (p0 >> p.cache.page_shift)];
-        ok = mbar_wait(&bars->empty[s], ((n / STAGES) & 1) ^ 1, abort_flag);
+        if (lane == 0) ok = mbar_wait(&bars->empty[s], ((n / STAGES) & 1) ^ 1, abort_flag);
+        ok = __shfl_sync(0xffffffffu, ok, 0);
         if (!ok) break;
-        unsigned char* dst = stage + off + (lo - t0) * bytes;
-        const int size = (hi - lo) * bytes;
-        if (copy && (unsigned)page < (unsigned)p.cache.pages) {
+        unsigned char* dst = smem + s * L::kStage + off + (c.lo - c.t0) * bytes;
+        const int size = (c.hi - c.lo) * bytes;
+        if (size > 0 && (unsigned)c.page < (unsigned)p.cache.pages) {
           mbar_arrive_expect_tx(&bars->full[s], size);
-          const int64_t row = (((int64_t)page * p.cache.Hk + hk) << p.cache.page_shift) + (lo & ((1 << p.cache.page_shift) - 1));
+          const int64_t row = (((int64_t)c.page * p.cache.Hk + hk) << p.cache.page_shift) + (c.lo & ((1 << p.cache.page_shift) - 1));
           bulk_load_1d(dst, src + row * bytes, size, &bars->full[s]);
         } else {
-          if (copy) {  // a page that does not exist: its keys are NaN
+          if (size > 0) {  // a page that does not exist: its keys are NaN
             bad = true;
             if (kind == 2) {
               for (int x = 0; x < size; x += 4) *reinterpret_cast<uint32_t*>(dst + x) = 0xffc0ffc0u;
@@ -485,27 +563,30 @@ __global__ void __launch_bounds__(CTA_THREADS, CTAS_PER_SM) cache_attn_kernel(co
     if (bad && p.status != nullptr) atomicOr(p.status, kBadPage);
   } else if (any) {
     // ------------------------------------------------------------ rows
+    // Scores are taken with keys as rows of the matrix instructions and queries as columns, outputs with elements as rows and
+    // queries as columns: 8 rows are an instruction's whole width.  Row i of 16 keys is token token_of(i) of the 16, an order in
+    // which the loads of keys meet no bank twice.  A lane's scores are those of tokens g and g + 8 with rows 2 t and 2 t + 1 (of 8);
+    // weights turn from there into columns' operands by movmatrix.
     const int g = lane >> 2, t = lane & 3;
-    // tokens of this lane's four columns of 16, and the key row that it loads for each block of eight columns
-    const int tok[4] = {t, (t ^ 1) + 4, t + 8, (t ^ 1) + 12};
-    const int krow = (g & 1) ? ((g >> 1) ^ 1) + 4 : g >> 1;
+    const int krow = (g & 1) ? ((g >> 1) ^ 1) + 4 : g >> 1;      // token_of(g); token_of(i + 8) = token_of(i) + 8
+    const int tok[4] = {t, (t ^ 1) + 4, t + 8, (t ^ 1) + 12};    // token_of(2 t), (2 t + 1), (2 t + 8), (2 t + 9)
     float* so = reinterpret_cast<float*>(smem + L::out_off) + warp * RT * L::kOutRow;
+    float2* table = reinterpret_cast<float2*>(so);
     float2* ml = reinterpret_cast<float2*>(smem + L::ml_off);
     int n = 0;
     bool ok = true;
     do {
       const int hk = w.item / p.row_blocks, r0 = (w.item % p.row_blocks) * RT, cnt = w.count();
-      // ---- the rows' queries as fp16 operands, and -8 sum of each group
-      uint32_t q[NG][2][4];
-      float qbias[NB][NG], f[NB];
-      int hi_row[NB], lo_row[NB];  // a row sees keys [lo_row, hi_row) and the sinks before hi_row
+      // ---- the rows' queries as fp16 operands, and -8 sum of each group; a lane loads row g of 8
+      uint32_t q[NB][NG][2][2];
+      uint64_t qbias[NB][NG];    // of rows 2 t and 2 t + 1, as f
+      float f[NB][2];
+      int hi_row[NB][2];         // a row sees keys [hi_row - window, hi_row) and the sinks before hi_row
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) {
         const int r = r0 + nb * 8 + g;
         const bool real = r < p.rows;
         const int head = r / p.M, i = r - head * p.M;
-        hi_row[nb] = real ? w.span.len - p.M + i + 1 : 0;
-        lo_row[nb] = hi_row[nb] - p.window;
         float x[NG][8];
         float top = 0.f;
         const T* qp = static_cast<const T*>(p.q) + w.b * p.q_sb + (int64_t)(hk * p.G + head) * p.q_sh + (int64_t)i * p.q_ss;
@@ -524,7 +605,14 @@ __global__ void __launch_bounds__(CTA_THREADS, CTAS_PER_SM) cache_attn_kernel(co
         k = max(-100, min(100, k));
         const float mul = __int_as_float((127 + k) << 23);
         // 2^22 undoes the subnormal; in two factors, so that neither leaves fp32's range
-        f[nb] = p.sm_scale * kLog2e * __int_as_float((127 + 22) << 23) * __int_as_float((127 - k) << 23);
+        const float my_f = p.sm_scale * kLog2e * __int_as_float((127 + 22) << 23) * __int_as_float((127 - k) << 23);
+        const int my_hi = real ? w.span.len - p.M + i + 1 : 0;
+        // rows 2 t and 2 t + 1 are loaded by the lanes 8 t and 8 t + 4
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          f[nb][c] = __shfl_sync(0xffffffffu, my_f, 8 * t + 4 * c);
+          hi_row[nb][c] = __shfl_sync(0xffffffffu, my_hi, 8 * t + 4 * c);
+        }
 #pragma unroll
         for (int gi = 0; gi < NG; ++gi) {
           float sum = 0.f;
@@ -536,23 +624,23 @@ __global__ void __launch_bounds__(CTA_THREADS, CTAS_PER_SM) cache_attn_kernel(co
           }
           sum += __shfl_xor_sync(0xffffffffu, sum, 1);
           sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-          qbias[nb][gi] = -8.f * 2.384185791015625e-7f * sum;
+          sum *= -8.f * 2.384185791015625e-7f;
+          qbias[nb][gi] = pack_f32x2(__shfl_sync(0xffffffffu, sum, 8 * t), __shfl_sync(0xffffffffu, sum, 8 * t + 4));
           auto pair = [&](int a, int b) {
             return (uint32_t)__half_as_ushort(h[a]) | (uint32_t)__half_as_ushort(h[b]) << 16;
           };
           // element y of a word is nibble y: registers (0, 4), (1, 5), (2, 6), (3, 7)
-          q[gi][0][nb] = pair(0, 4);
-          q[gi][0][2 + nb] = pair(1, 5);
-          q[gi][1][nb] = pair(2, 6);
-          q[gi][1][2 + nb] = pair(3, 7);
-          if (NB == 1) q[gi][0][1] = q[gi][0][3] = q[gi][1][1] = q[gi][1][3] = 0u;
+          q[nb][gi][0][0] = pair(0, 4);
+          q[nb][gi][0][1] = pair(1, 5);
+          q[nb][gi][1][0] = pair(2, 6);
+          q[nb][gi][1][1] = pair(3, 7);
         }
       }
-      float o[NB][NG][MT][4], ob[NB][NG][4], m[NB], l[NB];
+      float o[NB][NG][MT][4], ob[NB][NG][4], m[NB][2], l[NB][2];
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) {
-        m[nb] = FAWS_NEG_INF;
-        l[nb] = 0.f;
+        m[nb][0] = m[nb][1] = FAWS_NEG_INF;
+        l[nb][0] = l[nb][1] = 0.f;
 #pragma unroll
         for (int gi = 0; gi < NG; ++gi)
 #pragma unroll
@@ -564,160 +652,213 @@ __global__ void __launch_bounds__(CTA_THREADS, CTAS_PER_SM) cache_attn_kernel(co
       }
       const int hi_first = w.span.len - p.M + 1, lo_last = w.span.len - p.window;  // of the first, the last row
 
-      // ---- 16 tokens from `base` of the stage on, the first of them at position n0
+      // ---- 32 tokens from `base` of the stage on, the first of them at position n0, in two parts of 16; their scores come first, so
+      // that the maximum is looked at once
       auto step = [&](auto masked_tag, const unsigned char* stage, int base, int n0) {
         constexpr bool kMasked = decltype(masked_tag)::value;
-        float s[NB][4];
+        // Each lane converts one token's scales, each number twice, as the packed products want them.  Of the value scales also
+        // log2 of the token's largest, no less than -100 (a NaN, negative as an integer, has none).
+        float my_ev;
+        {
+          int top = 0x0d800000;  // 2^-100
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const unsigned char* kr = stage + L::k_off + (base + half * 8 + krow) * L::kRow;
-          uint32_t kw[NG];
-          if constexpr (NG == 4) *reinterpret_cast<uint4*>(kw) = *reinterpret_cast<const uint4*>(kr + t * 16);
-          else if constexpr (NG == 2) *reinterpret_cast<uint2*>(kw) = *reinterpret_cast<const uint2*>(kr + t * 8);
-          else if constexpr (D == 32) kw[0] = *reinterpret_cast<const uint32_t*>(kr + t * 4);
-          else kw[0] = (uint32_t)*reinterpret_cast<const uint16_t*>(kr + t * 2) << 2;  // elements 4 t .. + 3, then none
-          float acc[NG][4];
-#pragma unroll
-          for (int gi = 0; gi < NG; ++gi) {
-            acc[gi][0] = acc[gi][1] = qbias[0][gi];
-            acc[gi][2] = acc[gi][3] = NB == 2 ? qbias[NB - 1][gi] : 0.f;
-            const uint32_t lo = kw[gi], hi = __funnelshift_r(kw[gi], kw[gi], 8);
-            mma_f16(acc[gi], q[gi][0], lo & kLow, lo & kHigh);
-            mma_f16(acc[gi], q[gi][1], hi & kLow, hi & kHigh);
-          }
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const unsigned char* sp = stage + L::ks_off + (base + tok[half * 2 + e]) * L::kScale;
-            float sc[NG];
+          for (int kv = 0; kv < 2; ++kv) {
+            const unsigned char* sp = stage + (kv ? L::vs_off : L::ks_off) + (base + lane) * L::kScale;
+            float2* to = table + kv * (32 * NG) + lane * NG;
+            auto twice = [](float x) { return make_float2(x, x); };
             if constexpr (NG == 4) {
               const uint2 w2 = *reinterpret_cast<const uint2*>(sp);
-              sc[0] = bf16_lo(w2.x); sc[1] = bf16_hi(w2.x); sc[2] = bf16_lo(w2.y); sc[3] = bf16_hi(w2.y);
+              to[0] = twice(bf16_lo(w2.x)); to[1] = twice(bf16_hi(w2.x)); to[2] = twice(bf16_lo(w2.y)); to[3] = twice(bf16_hi(w2.y));
+              if (kv) {
+                const uint32_t mx = __vmaxs2(w2.x, w2.y);
+                top = max(max((int)(mx << 16), (int)(mx & 0xffff0000u)), top);
+              }
             } else if constexpr (NG == 2) {
               const uint32_t w1 = *reinterpret_cast<const uint32_t*>(sp);
-              sc[0] = bf16_lo(w1); sc[1] = bf16_hi(w1);
-            } else sc[0] = __uint_as_float((uint32_t)*reinterpret_cast<const uint16_t*>(sp) << 16);
-#pragma unroll
-            for (int nb = 0; nb < NB; ++nb) {
-              float x = sc[0] * acc[0][nb * 2 + e];
-#pragma unroll
-              for (int gi = 1; gi < NG; ++gi) x = fmaf(sc[gi], acc[gi][nb * 2 + e], x);
-              s[nb][half * 2 + e] = x * f[nb];
+              to[0] = twice(bf16_lo(w1)); to[1] = twice(bf16_hi(w1));
+              if (kv) top = max(max((int)(w1 << 16), (int)(w1 & 0xffff0000u)), top);
+            } else {
+              const uint32_t w1 = (uint32_t)*reinterpret_cast<const uint16_t*>(sp) << 16;
+              to[0] = twice(__uint_as_float(w1));
+              if (kv) top = max((int)w1, top);
             }
           }
+          my_ev = fast_log2(__int_as_float(top));
         }
-        if constexpr (kMasked) {
+        __syncwarp();
+        // scales (s, s) of the token `at` of the 32, group by group
+        auto scales = [&](int kv, int at, uint64_t (&sc)[NG]) {
+          const float2* from = table + kv * (32 * NG) + at * NG;
+          if constexpr (NG >= 2) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int j = n0 + tok[e];
+            for (int gi = 0; gi < NG; gi += 2) {
+              const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(from + gi);
+              sc[gi] = x.x;
+              sc[gi + 1] = x.y;
+            }
+          } else sc[0] = *reinterpret_cast<const uint64_t*>(from);
+        };
+        // scores without the rows' factors f: [part][rows nb * 8 + 2 t, + 1][token g, g + 8]
+        uint64_t s[2][NB][2];
 #pragma unroll
-            for (int nb = 0; nb < NB; ++nb)
-              if (!(j < hi_row[nb] && (j >= lo_row[nb] || j < p.sinks))) s[nb][e] = FAWS_NEG_INF;
+        for (int part = 0; part < 2; ++part) {
+          uint32_t kw[2][NG];
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const unsigned char* kr = stage + L::k_off + (base + part * 16 + half * 8 + krow) * L::kRow;
+            if constexpr (NG == 4) *reinterpret_cast<uint4*>(kw[half]) = *reinterpret_cast<const uint4*>(kr + t * 16);
+            else if constexpr (NG == 2) *reinterpret_cast<uint2*>(kw[half]) = *reinterpret_cast<const uint2*>(kr + t * 8);
+            else if constexpr (D == 32) kw[half][0] = *reinterpret_cast<const uint32_t*>(kr + t * 4);
+            else kw[half][0] = (uint32_t)*reinterpret_cast<const uint16_t*>(kr + t * 2) << 2;  // elements 4 t .. + 3, then none
           }
-        }
-        // ---- value scales, and about log2 of the largest of each token
-        float vs[4][NG], ev[4];
+          uint64_t sc[2][NG];
+          scales(0, part * 16 + krow, sc[0]);
+          scales(0, part * 16 + 8 + krow, sc[1]);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const unsigned char* sp = stage + L::vs_off + (base + tok[e]) * L::kScale;
-          int top;
-          if constexpr (NG == 4) {
-            const uint2 w2 = *reinterpret_cast<const uint2*>(sp);
-            vs[e][0] = bf16_lo(w2.x); vs[e][1] = bf16_hi(w2.x); vs[e][2] = bf16_lo(w2.y); vs[e][3] = bf16_hi(w2.y);
-            const uint32_t mx = __vmaxs2(w2.x, w2.y);
-            top = max((int)(mx << 16), (int)(mx & 0xffff0000u));
-          } else if constexpr (NG == 2) {
-            const uint32_t w1 = *reinterpret_cast<const uint32_t*>(sp);
-            vs[e][0] = bf16_lo(w1); vs[e][1] = bf16_hi(w1);
-            top = max((int)(w1 << 16), (int)(w1 & 0xffff0000u));
-          } else {
-            top = (int)((uint32_t)*reinterpret_cast<const uint16_t*>(sp) << 16);
-            vs[e][0] = __int_as_float(top);
-          }
-          // exponent and fraction of a float, read as an integer, are its log2 to 0.09; a NaN (negative) has none
-          ev[e] = fmaxf((float)top * 1.1920928955078125e-7f - 127.f, -100.f);
-        }
-        // ---- running maximum, moved only when a weighted value would exceed 2^8
-        bool need = false;
+          for (int gi = 0; gi < NG; ++gi) {
+            const uint32_t y0 = __funnelshift_r(kw[0][gi], kw[0][gi], 8), y1 = __funnelshift_r(kw[1][gi], kw[1][gi], 8);
+            const uint32_t a0[4] = {kw[0][gi] & kLow, kw[1][gi] & kLow, kw[0][gi] & kHigh, kw[1][gi] & kHigh};
+            const uint32_t a1[4] = {y0 & kLow, y1 & kLow, y0 & kHigh, y1 & kHigh};
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb) {
-          float mx = s[nb][0] + ev[0];
+            for (int nb = 0; nb < NB; ++nb) {
+              float acc[4];
+              mma_f16_first(acc, a0, q[nb][gi][0][0], q[nb][gi][0][1]);
+              mma_f16(acc, a1, q[nb][gi][1][0], q[nb][gi][1][1]);
 #pragma unroll
-          for (int e = 1; e < 4; ++e) mx = fmaxf(mx, s[nb][e] + ev[e]);
-          need = need || mx > m[nb] + 8.f;
-        }
-        if (__any_sync(0xffffffffu, need)) {
-#pragma unroll
-          for (int nb = 0; nb < NB; ++nb) {
-            float mx = s[nb][0] + ev[0];
-#pragma unroll
-            for (int e = 1; e < 4; ++e) mx = fmaxf(mx, s[nb][e] + ev[e]);
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-            const float m_new = fmaxf(m[nb], mx);
-            const float alpha = m_new == FAWS_NEG_INF ? 1.f : fast_exp2(m[nb] - m_new);
-            m[nb] = m_new;
-            l[nb] *= alpha;
-            // the outputs' columns 2 t and 2 t + 1 are rows of other lanes
-            const float a0 = __shfl_sync(0xffffffffu, alpha, t * 8), a1 = __shfl_sync(0xffffffffu, alpha, t * 8 + 4);
-#pragma unroll
-            for (int gi = 0; gi < NG; ++gi) {
-              ob[nb][gi][0] *= a0; ob[nb][gi][1] *= a1; ob[nb][gi][2] *= a0; ob[nb][gi][3] *= a1;
-#pragma unroll
-              for (int mt = 0; mt < MT; ++mt) {
-                o[nb][gi][mt][0] *= a0; o[nb][gi][mt][1] *= a1; o[nb][gi][mt][2] *= a0; o[nb][gi][mt][3] *= a1;
+              for (int half = 0; half < 2; ++half) {
+                const uint64_t x = add_f32x2(pack_f32x2(acc[2 * half], acc[2 * half + 1]), qbias[nb][gi]);
+                s[part][nb][half] = gi == 0 ? mul_f32x2(x, sc[half][gi]) : fma_f32x2(x, sc[half][gi], s[part][nb][half]);
               }
             }
           }
         }
-        float pr[NB][4];
+        // ---- running maximum, moved only when a weighted value would exceed 2^8
+        [[maybe_unused]] uint32_t hidden[NB];  // bit 4 part + 2 half + row
+        float top[NB][2], ev[2][2];
+        bool need = false;
+#pragma unroll
+        for (int part = 0; part < 2; ++part)
+#pragma unroll
+          for (int half = 0; half < 2; ++half) ev[part][half] = __shfl_sync(0xffffffffu, my_ev, part * 16 + half * 8 + krow);
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
-          const float ms = m[nb] == FAWS_NEG_INF ? 0.f : m[nb];
+          hidden[nb] = 0u;
+          float x[2][2][2];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            pr[nb][e] = fast_exp2(s[nb][e] - ms);
-            l[nb] += pr[nb][e];
+          for (int part = 0; part < 2; ++part)
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              float y[2];
+              unpack_f32x2(s[part][nb][half], y[0], y[1]);
+#pragma unroll
+              for (int c = 0; c < 2; ++c) {
+                x[c][part][half] = fmaf(y[c], f[nb][c], ev[part][half]);
+                if constexpr (kMasked) {
+                  const int j = n0 + part * 16 + half * 8 + krow;
+                  if (!(j < hi_row[nb][c] && (j >= hi_row[nb][c] - p.window || j < p.sinks))) {
+                    x[c][part][half] = FAWS_NEG_INF;
+                    hidden[nb] |= 1u << (part * 4 + half * 2 + c);
+                  }
+                }
+              }
+            }
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            top[nb][c] = fmax3(fmaxf(x[c][0][0], x[c][0][1]), x[c][1][0], x[c][1][1]);
+            need = need || top[nb][c] > m[nb][c] + 8.f;
           }
         }
-        // ---- values
-        uint32_t vw[4][(NG + 1) / 2];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const unsigned char* vr = stage + L::v_off + (base + tok[e]) * L::kRow;
-          if constexpr (NG == 4) *reinterpret_cast<uint2*>(vw[e]) = *reinterpret_cast<const uint2*>(vr + g * 8);
-          else if constexpr (NG == 2) vw[e][0] = *reinterpret_cast<const uint32_t*>(vr + g * 4);
-          else if constexpr (D == 32) vw[e][0] = *reinterpret_cast<const uint16_t*>(vr + g * 2);
-          else vw[e][0] = vr[g];
-        }
-#pragma unroll
-        for (int gi = 0; gi < NG; ++gi) {
-          // both tokens' half-words of the group; then with their bytes exchanged, which brings the next two nibbles
-          const uint32_t sel = (gi & 1) ? 0x7632u : 0x5410u, swapped = (gi & 1) ? 0x6723u : 0x4501u;
-          uint32_t x01 = __byte_perm(vw[0][gi >> 1], vw[1][gi >> 1], sel), x23 = __byte_perm(vw[2][gi >> 1], vw[3][gi >> 1], sel);
-          if (D == 16) {
-            x01 <<= 2;
-            x23 <<= 2;
-          }
-          const uint32_t a0[4] = {x01 & kLow, x01 & kHigh, x23 & kLow, x23 & kHigh};
-          const uint32_t ab[4] = {0x00200020u, 0x02000200u, 0x00200020u, 0x02000200u};  // 8 in every place
-          [[maybe_unused]] uint32_t a1[4];
-          if constexpr (MT == 2) {
-            const uint32_t y01 = __byte_perm(vw[0][gi >> 1], vw[1][gi >> 1], swapped);
-            const uint32_t y23 = __byte_perm(vw[2][gi >> 1], vw[3][gi >> 1], swapped);
-            a1[0] = y01 & kLow; a1[1] = y01 & kHigh; a1[2] = y23 & kLow; a1[3] = y23 & kHigh;
-          }
+        if (__any_sync(0xffffffffu, need)) {
 #pragma unroll
           for (int nb = 0; nb < NB; ++nb) {
-            float pv[4];
+            float alpha[2];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              pv[e] = pr[nb][e] * vs[e][gi];
-              if (kMasked && pr[nb][e] == 0.f) pv[e] = 0.f;  // a hidden token's scale may be anything
+            for (int c = 0; c < 2; ++c) {
+              float mx = top[nb][c];
+#pragma unroll
+              for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+              const float m_new = fmaxf(m[nb][c], mx);
+              alpha[c] = m_new == FAWS_NEG_INF ? 1.f : fast_exp2(m[nb][c] - m_new);
+              m[nb][c] = m_new;
+              l[nb][c] *= alpha[c];
             }
-            const uint32_t b0 = pack2<__half>(pv[0], pv[1]), b1 = pack2<__half>(pv[2], pv[3]);
-            mma_f16(o[nb][gi][0], a0, b0, b1);
-            if constexpr (MT == 2) mma_f16(o[nb][gi][MT - 1], a1, b0, b1);
-            mma_f16(ob[nb][gi], ab, b0, b1);
+#pragma unroll
+            for (int gi = 0; gi < NG; ++gi)
+#pragma unroll
+              for (int c = 0; c < 4; ++c) {
+                ob[nb][gi][c] *= alpha[c & 1];
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) o[nb][gi][mt][c] *= alpha[c & 1];
+              }
+          }
+        }
+        // ---- weights, and values
+#pragma unroll
+        for (int part = 0; part < 2; ++part) {
+          uint64_t pr[NB][2];  // [token g, g + 8], rows 2 t and 2 t + 1
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              float y[2];
+              unpack_f32x2(s[part][nb][half], y[0], y[1]);
+#pragma unroll
+              for (int c = 0; c < 2; ++c) {
+                y[c] = fast_exp2(fmaf(y[c], f[nb][c], m[nb][c] == FAWS_NEG_INF ? 0.f : -m[nb][c]));
+                if (kMasked && (hidden[nb] >> (part * 4 + half * 2 + c) & 1u)) y[c] = 0.f;
+                l[nb][c] += y[c];
+              }
+              pr[nb][half] = pack_f32x2(y[0], y[1]);
+            }
+          }
+          uint64_t vs[2][NG];
+          scales(1, part * 16 + krow, vs[0]);
+          scales(1, part * 16 + 8 + krow, vs[1]);
+          uint32_t vw[4][(NG + 1) / 2];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const unsigned char* vr = stage + L::v_off + (base + part * 16 + tok[e]) * L::kRow;
+            if constexpr (NG == 4) *reinterpret_cast<uint2*>(vw[e]) = *reinterpret_cast<const uint2*>(vr + g * 8);
+            else if constexpr (NG == 2) vw[e][0] = *reinterpret_cast<const uint32_t*>(vr + g * 4);
+            else if constexpr (D == 32) vw[e][0] = *reinterpret_cast<const uint16_t*>(vr + g * 2);
+            else vw[e][0] = vr[g];
+          }
+#pragma unroll
+          for (int gi = 0; gi < NG; ++gi) {
+            // both tokens' half-words of the group; then with their bytes exchanged, which brings the next two nibbles
+            const uint32_t sel = (gi & 1) ? 0x7632u : 0x5410u;
+            [[maybe_unused]] const uint32_t swapped = (gi & 1) ? 0x6723u : 0x4501u;
+            uint32_t x01 = __byte_perm(vw[0][gi >> 1], vw[1][gi >> 1], sel), x23 = __byte_perm(vw[2][gi >> 1], vw[3][gi >> 1], sel);
+            if (D == 16) {
+              x01 <<= 2;
+              x23 <<= 2;
+            }
+            const uint32_t a0[4] = {x01 & kLow, x01 & kHigh, x23 & kLow, x23 & kHigh};
+            const uint32_t ab[4] = {0x00200020u, 0x02000200u, 0x00200020u, 0x02000200u};  // 8 in every place
+            [[maybe_unused]] uint32_t a1[4];
+            if constexpr (MT == 2) {
+              const uint32_t y01 = __byte_perm(vw[0][gi >> 1], vw[1][gi >> 1], swapped);
+              const uint32_t y23 = __byte_perm(vw[2][gi >> 1], vw[3][gi >> 1], swapped);
+              a1[0] = y01 & kLow; a1[1] = y01 & kHigh; a1[2] = y23 & kLow; a1[3] = y23 & kHigh;
+            }
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) {
+              uint32_t pb[2];
+#pragma unroll
+              for (int half = 0; half < 2; ++half) {
+                float pv[2];
+                unpack_f32x2(mul_f32x2(pr[nb][half], vs[half][gi]), pv[0], pv[1]);
+                if constexpr (kMasked) {  // a hidden token's scale may be anything
+#pragma unroll
+                  for (int c = 0; c < 2; ++c)
+                    if (hidden[nb] >> (part * 4 + half * 2 + c) & 1u) pv[c] = 0.f;
+                }
+                pb[half] = transpose8(pack2<__half>(pv[0], pv[1]));
+              }
+              mma_f16(o[nb][gi][0], a0, pb[0], pb[1]);
+              if constexpr (MT == 2) mma_f16(o[nb][gi][MT - 1], a1, pb[0], pb[1]);
+              mma_f16(ob[nb][gi], ab, pb[0], pb[1]);
+            }
           }
         }
       };
@@ -730,15 +871,8 @@ __global__ void __launch_bounds__(CTA_THREADS, CTAS_PER_SM) cache_attn_kernel(co
         const int n0 = t0 + warp * 32;
         const bool whole = n0 + 32 <= hi_first && (n0 >= lo_last || n0 + 32 <= p.sinks);
         // (32 tokens that no row sees are skipped)
-        if (whole) {
-          step(std::false_type{}, stage, warp * 32, n0);
-          step(std::false_type{}, stage, warp * 32 + 16, n0 + 16);
-        } else {
-#pragma unroll 1
-          for (int x = 0; x < 32; x += 16)
-            if (n0 + x < w.span.len && (n0 + x + 16 > w.span.lo || n0 + x < p.sinks))
-              step(std::true_type{}, stage, warp * 32 + x, n0 + x);
-        }
+        if (whole) step(std::false_type{}, stage, warp * 32, n0);
+        else if (n0 < w.span.len && (n0 + 32 > w.span.lo || n0 < p.sinks)) step(std::true_type{}, stage, warp * 32, n0);
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars->empty[st]);
       }
@@ -746,10 +880,13 @@ __global__ void __launch_bounds__(CTA_THREADS, CTAS_PER_SM) cache_attn_kernel(co
       // ---- the four warps' parts
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) {
-        float ls = l[nb];
-        ls += __shfl_xor_sync(0xffffffffu, ls, 1);
-        ls += __shfl_xor_sync(0xffffffffu, ls, 2);
-        if (t == 0) ml[warp * RT + nb * 8 + g] = make_float2(m[nb], ls);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          float ls = l[nb][c];
+#pragma unroll
+          for (int x = 4; x < 32; x <<= 1) ls += __shfl_xor_sync(0xffffffffu, ls, x);
+          if (g == 0) ml[warp * RT + nb * 8 + 2 * t + c] = make_float2(m[nb][c], ls);
+        }
 #pragma unroll
         for (int gi = 0; gi < NG; ++gi)
 #pragma unroll
@@ -898,22 +1035,26 @@ cudaError_t launch_attn_t(const CacheAttnParams& p, cudaStream_t s) {
   }
 }
 
-int shares_at_most() { return CTAS_PER_SM * sm_count(); }
+int shares_at_most(int rows) { return ctas_per_sm(rows <= 8 ? 8 : 16) * sm_count(); }
 
+template <typename T, bool WRITE, int D>
+cudaError_t launch_rows_d(const CacheParams& c, const CacheBatch& b, CacheRows r, cudaStream_t s) {
+  // few rows (decoding): small CTAs, so that heads and sequences fill the chip
+  int lanes = 32 / (D / 8) > 1 ? 32 / (D / 8) : 1;
+  while (lanes * (D / 8) < 256 && lanes * kRowsEach < r.rows) lanes *= 2;
+  r.tiles = (r.rows + lanes * kRowsEach - 1) / (lanes * kRowsEach);
+  const dim3 grid((unsigned)((int64_t)b.B * c.Hk * r.tiles), 2, 1);
+  return launch_overlapped(WRITE ? cache_write_kernel<T, D> : cache_read_kernel<T, D>, grid, lanes * (D / 8), 0, s, c, b, r,
+                           tc_status_word());
+}
 template <typename T, bool WRITE>
 cudaError_t launch_rows_t(const CacheParams& c, const CacheBatch& b, const CacheRows& r, cudaStream_t s) {
-  const int64_t threads = (int64_t)b.B * c.Hk * r.rows * (c.D / 8);
-  const dim3 grid((unsigned)((threads + 255) / 256), 2, 1);
-  int* status = tc_status_word();
-#define FAWS_ROWS(D)                                                                          \
-  return launch_overlapped(WRITE ? cache_write_kernel<T, D> : cache_read_kernel<T, D>, grid, 256, 0, s, c, b, r, status)
   switch (c.D) {
-    case 16: FAWS_ROWS(16);
-    case 32: FAWS_ROWS(32);
-    case 64: FAWS_ROWS(64);
-    default: FAWS_ROWS(128);
+    case 16: return launch_rows_d<T, WRITE, 16>(c, b, r, s);
+    case 32: return launch_rows_d<T, WRITE, 32>(c, b, r, s);
+    case 64: return launch_rows_d<T, WRITE, 64>(c, b, r, s);
+    default: return launch_rows_d<T, WRITE, 128>(c, b, r, s);
   }
-#undef FAWS_ROWS
 }
 
 CacheRows make_rows(const faws_tensor* k, const faws_tensor* v, int rows, bool write) {
@@ -947,12 +1088,12 @@ cudaError_t launch_cache_read(const CacheParams& c, const CacheBatch& b, const f
 }
 
 size_t cache_attn_workspace_bytes(int rows, int D) {
-  return (size_t)shares_at_most() * 2 * (rows <= 8 ? 8 : 16) * (D + 2) * 4;
+  return (size_t)shares_at_most(rows) * 2 * (rows <= 8 ? 8 : 16) * (D + 2) * 4;
 }
 
 cudaError_t launch_cache_attn(const CacheAttnParams& call, int dtype, cudaStream_t s) {
   CacheAttnParams p = call;
-  p.grid = shares_at_most();
+  p.grid = shares_at_most(p.rows);
   p.min_tiles = 2;
   p.vec_out = reinterpret_cast<uintptr_t>(p.out) % 8 == 0 && p.o_sb % 4 == 0 && p.o_sh % 4 == 0 && p.o_ss % 4 == 0;
   p.status = tc_status_word();
