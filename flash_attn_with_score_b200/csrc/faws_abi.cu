@@ -878,8 +878,7 @@ int faws_kv_cache_read(const faws_kv_cache* c, const faws_cache_batch* batch, co
 size_t faws_kv_cache_workspace_bytes(const faws_problem* p) {
   if (p == nullptr || p->B <= 0 || p->Hq <= 0 || p->Hk <= 0 || p->M <= 0 || p->Hq % p->Hk != 0) return 0;
   if (p->D != 16 && p->D != 32 && p->D != 64 && p->D != 128) return 0;
-  const int64_t rows = (int64_t)(p->Hq / p->Hk) * p->M;
-  return align256(cache_attn_workspace_bytes(rows > 8 ? 16 : 8, p->D));
+  return align256(cache_attn_workspace_bytes(p->D));
 }
 
 int faws_attention_with_kv_cache(const faws_problem* p, const faws_kv_cache* c, const faws_cache_batch* batch,
@@ -890,6 +889,9 @@ int faws_attention_with_kv_cache(const faws_problem* p, const faws_kv_cache* c, 
   if (st != FAWS_OK) return st;
   if (p->B != batch->B || p->Hk != c->Hk || p->D != c->D || p->dtype != c->dtype) return FAWS_EINVAL;
   if (p->q.ptr == nullptr || p->out.ptr == nullptr || window < 0 || sinks < 0 || rows > (1 << 30)) return FAWS_EINVAL;
+  // the kernel counts tiles of 128 tokens in 32 bits
+  const int64_t tiles = ((int64_t)batch->max_pages * c->page_size + 127) / 128;
+  if (tiles * ((rows + 7) / 8) > ((int64_t(1) << 31) - 1) / ((int64_t)p->B * p->Hk)) return FAWS_EINVAL;
   if (workspace == nullptr || workspace_bytes < faws_kv_cache_workspace_bytes(p) || misaligned_ws(workspace)) return FAWS_EWORKSPACE;
   CacheAttnParams a{};
   a.cache = make_cache(c);

@@ -274,7 +274,7 @@ __global__ void __launch_bounds__(256) cache_read_kernel(CacheParams c, CacheBat
 }
 
 // ---------------------------------------------------------------------------------------------- attention
-// One kv head's RT rows (the M query rows of each of its G query heads, one head after the other, 8 or 16 at a time)
+// One kv head's rows (the M query rows of each of its G query heads, one head after the other), 8 at a time,
 // against the tokens they see, in tiles of 128.  The bytes of the cache bound it, so the tiles of all sequences and heads
 // are one list that is cut into equal shares, a CTA each: lengths are on the device, and no share waits for the longest
 // sequence.  What a share has of an item (a row block) that it does not finish goes to the workspace, and a second kernel
@@ -293,11 +293,12 @@ __global__ void __launch_bounds__(256) cache_read_kernel(CacheParams c, CacheBat
 //                                                  matrix instruction per group, with the same rounded weights.
 // Weights are fp16: 2^-12 of each.  The running maximum is that of S + log2 s, so that P s stays within fp16 for values of
 // any size; what falls below 2^-24 of the largest weighted value is lost.
+constexpr int RT = 8;         // rows of a row block: the width of a matrix instruction
 constexpr int TT = 128;       // tokens of a tile
 constexpr int STAGES = 3;
 constexpr int CONSUMERS = 4;  // warps
 constexpr int CTA_THREADS = 32 * (CONSUMERS + 1);
-__host__ __device__ constexpr int ctas_per_sm(int rt) { return rt == 8 ? 3 : 2; }
+constexpr int CTAS_PER_SM = 3;
 constexpr uint32_t kLow = 0x003c003cu, kHigh = 0x03c003c0u;  // the two nibbles of each half's mantissa
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -348,67 +349,68 @@ __device__ __forceinline__ Span span_of(const CacheAttnParams& p, int b, bool* b
   return s;
 }
 
-// The tiles of all items (b, kv head, row block) in a row, cut into `shares`.
+// The tiles of all items (b, kv head, row block) in a row, cut into `shares` that differ by one at most.  (The entry point keeps
+// the list below 2^31 tiles.)
 struct Shares {
-  long long total;
-  int shares;
-  __device__ __forceinline__ long long begin(int c) const { return total * c / shares; }
-};
-// Warp-wide.  With `find`: the sequence that holds tile `find` of the list, and the list's index of its first tile.
-__device__ __forceinline__ long long scan_tiles(const CacheAttnParams& p, int lane, long long find, int* b_found,
-                                                long long* b_start) {
-  long long base = 0;
-  const int per = p.cache.Hk * p.row_blocks;
-  bool bad = false;
-  for (int b0 = 0; b0 < p.batch.B; b0 += 32) {
-    const int b = b0 + lane;
-    long long n = b < p.batch.B ? (long long)span_of(p, b, &bad).nt * per : 0;
-#pragma unroll
-    for (int s = 1; s < 32; s <<= 1) {
-      const long long up = __shfl_up_sync(0xffffffffu, n, s);
-      if (lane >= s) n += up;
-    }
-    if (find >= 0) {
-      const unsigned past = __ballot_sync(0xffffffffu, base + n > find);
-      if (past != 0u) {
-        const int first = __ffs(past) - 1;
-        const long long before = __shfl_up_sync(0xffffffffu, n, 1);
-        *b_start = base + (first == 0 ? 0 : __shfl_sync(0xffffffffu, before, first));
-        *b_found = b0 + first;
-        return -1;
-      }
-    }
-    base += __shfl_sync(0xffffffffu, n, 31);
+  int shares, per, more;  // the first `more` shares have one tile more
+  Shares() = default;
+  __device__ __forceinline__ Shares(const CacheAttnParams& p, int total) {
+    shares = max(1, min(p.grid, (total + p.min_tiles - 1) / p.min_tiles));
+    per = total / shares;
+    more = total - per * shares;
   }
-  if (bad && p.status != nullptr) atomicOr(p.status, kBadPage);
-  return base;
-}
-__device__ __forceinline__ Shares make_shares(const CacheAttnParams& p, long long total) {
-  const long long most = (total + p.min_tiles - 1) / p.min_tiles;
-  return {total, (int)max(1ll, min((long long)p.grid, most))};
-}
+  __device__ __forceinline__ int begin(int c) const { return c * per + min(c, more); }
+  __device__ __forceinline__ int of(int tile) const {
+    const int cut = more * (per + 1);
+    return tile < cut ? tile / (per + 1) : more + (tile - cut) / per;
+  }
+};
 
 // A share's walk over its segments, each some tiles of one item.
 struct Walk {
-  long long at, end;  // in the list of tiles
-  int b, item;        // item: kv head * row_blocks + row block
-  int first;          // first tile of the segment within its item
+  int at, end;  // in the list of tiles
+  int b, item;  // item: kv head * row_blocks + row block
+  int first;    // first tile of the segment within its item
   Span span;
-  __device__ __forceinline__ int count() const { return (int)min((long long)(span.nt - first), end - at); }
+  __device__ __forceinline__ int count() const { return min(span.nt - first, end - at); }
 };
-__device__ __forceinline__ bool walk_begin(const CacheAttnParams& p, int lane, Walk* w) {
-  const Shares sh = make_shares(p, scan_tiles(p, lane, -1, nullptr, nullptr));
-  if ((int)blockIdx.x >= sh.shares) return false;
-  w->at = sh.begin(blockIdx.x);
-  w->end = sh.begin(blockIdx.x + 1);
-  if (w->at >= w->end) return false;
-  long long start = 0;
-  scan_tiles(p, lane, w->at, &w->b, &start);
+// The CTA's first segment, by one warp.  false: the share is empty.
+__device__ __forceinline__ bool walk_begin(const CacheAttnParams& p, int lane, Walk* w, Shares* shares) {
+  const int items = p.cache.Hk * p.row_blocks;
   bool bad = false;
-  w->span = span_of(p, w->b, &bad);
-  const long long off = w->at - start;
-  w->item = (int)(off / w->span.nt);
-  w->first = (int)(off % w->span.nt);
+  int total = 0, n = 0;  // n: tiles of the sequences of a chunk of 32 up to this lane's
+  auto chunk = [&](int b0) {
+    n = b0 + lane < p.batch.B ? span_of(p, b0 + lane, &bad).nt * items : 0;
+#pragma unroll
+    for (int s = 1; s < 32; s <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, n, s);
+      if (lane >= s) n += up;
+    }
+    return __shfl_sync(0xffffffffu, n, 31);
+  };
+  for (int b0 = 0; b0 < p.batch.B; b0 += 32) total += chunk(b0);
+  if (bad && p.status != nullptr) atomicOr(p.status, kBadPage);
+  const Shares sh(p, total);
+  *shares = sh;
+  w->at = sh.begin(min((int)blockIdx.x, sh.shares));
+  w->end = sh.begin(min((int)blockIdx.x + 1, sh.shares));
+  if (w->at >= w->end) return false;
+  int base = 0;
+  for (int b0 = 0;; b0 += 32) {
+    const int all = p.batch.B <= 32 ? total : chunk(b0);  // (one chunk: as it was)
+    const unsigned past = __ballot_sync(0xffffffffu, base + n > w->at);
+    if (past != 0u) {
+      const int first = __ffs(past) - 1;
+      const int before = __shfl_sync(0xffffffffu, n, max(first - 1, 0));
+      w->b = b0 + first;
+      w->span = span_of(p, w->b, &bad);
+      const int off = w->at - base - (first == 0 ? 0 : before);
+      w->item = off / w->span.nt;
+      w->first = off - w->item * w->span.nt;
+      break;
+    }
+    base += all;
+  }
   return true;
 }
 __device__ __forceinline__ bool walk_next(const CacheAttnParams& p, Walk* w) {
@@ -426,7 +428,7 @@ __device__ __forceinline__ bool walk_next(const CacheAttnParams& p, Walk* w) {
   return true;
 }
 
-template <int D, int RT>
+template <int D>
 struct CacheSmem {
   static constexpr int NG = D >= 32 ? D / 32 : 1;
   static constexpr int kRow = D / 2, kScale = NG * 2;  // bytes of a token
@@ -438,20 +440,24 @@ struct CacheSmem {
   static constexpr int bar_off = ml_off + CONSUMERS * RT * 8;
   // While a segment lasts a warp's part of the output area holds its 32 tokens' scales of keys and values as pairs of floats.
   static_assert(2 * 32 * NG * 8 <= RT * kOutRow * 4, "room for the scales");
-  static constexpr int total = bar_off + 128;
+  static constexpr int total = bar_off + 192;
 };
 struct CacheBars {
   uint64_t full[STAGES], empty[STAGES];
-  int abort_flag;
+  int abort_flag, any;
+  Walk walk;  // where the CTA begins
+  Shares shares;
 };
-static_assert(sizeof(CacheBars) <= 128, "room for the barriers");
+static_assert(sizeof(CacheBars) <= 192, "room for the barriers");
 
-// Workspace: per share two slots of RT rows: D floats, then the row's maximum (log2 units) and sum.
-// Slot 0: the share's first segment, where it does not begin its item; slot 1: the last, where it begins its item but does not end it.
-template <int D, int RT>
-__device__ __forceinline__ float* part_slot(float* ws, int share, int slot) {
-  return ws + ((int64_t)share * 2 + slot) * RT * (D + 2);
+// Workspace: a header per share, then two slots of RT rows: D floats, the row's maximum (log2 units) and sum, and 2 floats unused.
+// Slot 0: the share's first segment, where it does not begin its item; slot 1: the last, where it begins its item but does not
+// end it.  The header tells what slot 1 is the beginning of: sequence, item, and the share that ends it, -1 where there is none.
+template <int D>
+__device__ __forceinline__ float* part_slot(const CacheAttnParams& p, int share, int slot) {
+  return p.parts + p.grid * 4 + ((int64_t)share * 2 + slot) * RT * (D + 4);
 }
+__device__ __forceinline__ int4* part_header(const CacheAttnParams& p, int share) { return reinterpret_cast<int4*>(p.parts) + share; }
 
 // Four elements of a finished row: sum / den, zeros for a row that saw nothing.
 template <typename T>
@@ -470,9 +476,9 @@ __device__ __forceinline__ void store_row(const CacheAttnParams& p, int b, int h
     p.L[((int64_t)b * p.G * p.cache.Hk + head) * p.M + i] = den == 0.f ? FAWS_NEG_INF : fmaf(top, kLn2, logf(den));
 }
 
-template <typename T, int D, int RT>
-__global__ void __launch_bounds__(CTA_THREADS, ctas_per_sm(RT)) cache_attn_kernel(const CacheAttnParams p) {
-  using L = CacheSmem<D, RT>;
+template <typename T, int D>
+__global__ void __launch_bounds__(CTA_THREADS, CTAS_PER_SM) cache_attn_kernel(const CacheAttnParams p) {
+  using L = CacheSmem<D>;
   constexpr int NG = L::NG;
   constexpr int MT = D >= 32 ? 2 : 1;  // 16-row tiles of a group's output
   constexpr int NB = RT / 8;           // blocks of 8 rows
@@ -491,8 +497,29 @@ __global__ void __launch_bounds__(CTA_THREADS, ctas_per_sm(RT)) cache_attn_kerne
   __syncthreads();
   griddep_wait();
   griddep_launch_dependents();
-  Walk w;
-  const bool any = walk_begin(p, lane, &w);  // (the same in every warp)
+  if (warp == 0) {
+    Walk first;
+    Shares shares;
+    const bool some = walk_begin(p, lane, &first, &shares);
+    if (lane == 0) {
+      bars->any = some ? 1 : 0;
+      bars->walk = first;
+      bars->shares = shares;
+    }
+  } else if (warp == 1) {  // sequences without a key have no tiles: their rows are zero
+    for (int b = blockIdx.x; b < p.batch.B; b += gridDim.x) {
+      bool bad = false;
+      if (span_of(p, b, &bad).nt > 0) continue;
+      for (int x = lane; x < p.cache.Hk * p.rows * (D / 4); x += 32) {
+        const int row = x / (D / 4), hk = row / p.rows;
+        store_row<T>(p, b, hk, row - hk * p.rows, (x % (D / 4)) * 4, make_float4(0.f, 0.f, 0.f, 0.f), 0.f, 0.f);
+      }
+    }
+  }
+  __syncthreads();
+  const bool any = bars->any != 0;
+  Walk w = bars->walk;
+  if (!any && threadIdx.x == 0) part_header(p, blockIdx.x)->w = -1;
 
   if (any && warp == CONSUMERS) {
     // ------------------------------------------------------------ copies
@@ -571,7 +598,7 @@ __global__ void __launch_bounds__(CTA_THREADS, ctas_per_sm(RT)) cache_attn_kerne
     const int krow = (g & 1) ? ((g >> 1) ^ 1) + 4 : g >> 1;      // token_of(g); token_of(i + 8) = token_of(i) + 8
     const int tok[4] = {t, (t ^ 1) + 4, t + 8, (t ^ 1) + 12};    // token_of(2 t), (2 t + 1), (2 t + 8), (2 t + 9)
     float* so = reinterpret_cast<float*>(smem + L::out_off) + warp * RT * L::kOutRow;
-    float2* table = reinterpret_cast<float2*>(so);
+    float4* table = reinterpret_cast<float4*>(so);  // [keys, values][pair of groups][token]
     float2* ml = reinterpret_cast<float2*>(smem + L::ml_off);
     int n = 0;
     bool ok = true;
@@ -664,22 +691,24 @@ __global__ void __launch_bounds__(CTA_THREADS, ctas_per_sm(RT)) cache_attn_kerne
 #pragma unroll
           for (int kv = 0; kv < 2; ++kv) {
             const unsigned char* sp = stage + (kv ? L::vs_off : L::ks_off) + (base + lane) * L::kScale;
-            float2* to = table + kv * (32 * NG) + lane * NG;
-            auto twice = [](float x) { return make_float2(x, x); };
+            using Entry = typename std::conditional<NG == 1, float2, float4>::type;
+            Entry* to = reinterpret_cast<Entry*>(table) + kv * 32 * ((NG + 1) / 2) + lane;
+            auto twice = [](uint32_t w) { return make_float4(bf16_lo(w), bf16_lo(w), bf16_hi(w), bf16_hi(w)); };
             if constexpr (NG == 4) {
               const uint2 w2 = *reinterpret_cast<const uint2*>(sp);
-              to[0] = twice(bf16_lo(w2.x)); to[1] = twice(bf16_hi(w2.x)); to[2] = twice(bf16_lo(w2.y)); to[3] = twice(bf16_hi(w2.y));
+              to[0] = twice(w2.x);
+              to[32] = twice(w2.y);
               if (kv) {
                 const uint32_t mx = __vmaxs2(w2.x, w2.y);
                 top = max(max((int)(mx << 16), (int)(mx & 0xffff0000u)), top);
               }
             } else if constexpr (NG == 2) {
               const uint32_t w1 = *reinterpret_cast<const uint32_t*>(sp);
-              to[0] = twice(bf16_lo(w1)); to[1] = twice(bf16_hi(w1));
+              to[0] = twice(w1);
               if (kv) top = max(max((int)(w1 << 16), (int)(w1 & 0xffff0000u)), top);
             } else {
               const uint32_t w1 = (uint32_t)*reinterpret_cast<const uint16_t*>(sp) << 16;
-              to[0] = twice(__uint_as_float(w1));
+              to[0] = make_float2(__uint_as_float(w1), __uint_as_float(w1));
               if (kv) top = max((int)w1, top);
             }
           }
@@ -688,15 +717,15 @@ __global__ void __launch_bounds__(CTA_THREADS, ctas_per_sm(RT)) cache_attn_kerne
         __syncwarp();
         // scales (s, s) of the token `at` of the 32, group by group
         auto scales = [&](int kv, int at, uint64_t (&sc)[NG]) {
-          const float2* from = table + kv * (32 * NG) + at * NG;
           if constexpr (NG >= 2) {
+            const float4* from = table + kv * 32 * (NG / 2) + at;
 #pragma unroll
             for (int gi = 0; gi < NG; gi += 2) {
-              const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(from + gi);
+              const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(from + gi / 2 * 32);
               sc[gi] = x.x;
               sc[gi + 1] = x.y;
             }
-          } else sc[0] = *reinterpret_cast<const uint64_t*>(from);
+          } else sc[0] = reinterpret_cast<const uint64_t*>(table)[kv * 32 + at];
         };
         // scores without the rows' factors f: [part][rows nb * 8 + 2 t, + 1][token g, g + 8]
         uint64_t s[2][NB][2];
@@ -823,6 +852,23 @@ __global__ void __launch_bounds__(CTA_THREADS, ctas_per_sm(RT)) cache_attn_kerne
             else if constexpr (D == 32) vw[e][0] = *reinterpret_cast<const uint16_t*>(vr + g * 2);
             else vw[e][0] = vr[g];
           }
+          // the weighted scales as operands, all of them before the products that wait for them
+          uint32_t pb[NB][NG][2];
+#pragma unroll
+          for (int gi = 0; gi < NG; ++gi)
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+              for (int half = 0; half < 2; ++half) {
+                float pv[2];
+                unpack_f32x2(mul_f32x2(pr[nb][half], vs[half][gi]), pv[0], pv[1]);
+                if constexpr (kMasked) {  // a hidden token's scale may be anything
+#pragma unroll
+                  for (int c = 0; c < 2; ++c)
+                    if (hidden[nb] >> (part * 4 + half * 2 + c) & 1u) pv[c] = 0.f;
+                }
+                pb[nb][gi][half] = transpose8(pack2<__half>(pv[0], pv[1]));
+              }
 #pragma unroll
           for (int gi = 0; gi < NG; ++gi) {
             // both tokens' half-words of the group; then with their bytes exchanged, which brings the next two nibbles
@@ -843,21 +889,9 @@ __global__ void __launch_bounds__(CTA_THREADS, ctas_per_sm(RT)) cache_attn_kerne
             }
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
-              uint32_t pb[2];
-#pragma unroll
-              for (int half = 0; half < 2; ++half) {
-                float pv[2];
-                unpack_f32x2(mul_f32x2(pr[nb][half], vs[half][gi]), pv[0], pv[1]);
-                if constexpr (kMasked) {  // a hidden token's scale may be anything
-#pragma unroll
-                  for (int c = 0; c < 2; ++c)
-                    if (hidden[nb] >> (part * 4 + half * 2 + c) & 1u) pv[c] = 0.f;
-                }
-                pb[half] = transpose8(pack2<__half>(pv[0], pv[1]));
-              }
-              mma_f16(o[nb][gi][0], a0, pb[0], pb[1]);
-              if constexpr (MT == 2) mma_f16(o[nb][gi][MT - 1], a1, pb[0], pb[1]);
-              mma_f16(ob[nb][gi], ab, pb[0], pb[1]);
+              mma_f16(o[nb][gi][0], a0, pb[nb][gi][0], pb[nb][gi][1]);
+              if constexpr (MT == 2) mma_f16(o[nb][gi][MT - 1], a1, pb[nb][gi][0], pb[nb][gi][1]);
+              mma_f16(ob[nb][gi], ab, pb[nb][gi][0], pb[nb][gi][1]);
             }
           }
         }
@@ -919,10 +953,14 @@ __global__ void __launch_bounds__(CTA_THREADS, ctas_per_sm(RT)) cache_attn_kerne
         if (begins && ends) {
           store_row<T>(p, w.b, hk, r0 + row, d, sum, top, den);
         } else {
-          float* part = part_slot<D, RT>(p.parts, blockIdx.x, begins ? 1 : 0) + row * (D + 2);
-          part[d] = sum.x; part[d + 1] = sum.y; part[d + 2] = sum.z; part[d + 3] = sum.w;
-          if (d == 0) { part[D] = top; part[D + 1] = den; }
+          float* part = part_slot<D>(p, blockIdx.x, begins ? 1 : 0) + row * (D + 4);
+          *reinterpret_cast<float4*>(part + d) = sum;
+          if (d == 0) *reinterpret_cast<float2*>(part + D) = make_float2(top, den);
         }
+      }
+      if (threadIdx.x == 0 && w.at + cnt >= w.end) {  // the share's last segment
+        const int end = begins && !ends ? bars->shares.of(w.at + w.span.nt - 1) : -1;
+        *part_header(p, blockIdx.x) = make_int4(w.b, w.item, 0, end);
       }
       ok = !consumers_any(!ok);  // (all of them go on, or none)
     } while (ok && walk_next(p, &w));
@@ -935,60 +973,49 @@ __global__ void __launch_bounds__(CTA_THREADS, ctas_per_sm(RT)) cache_attn_kerne
   }
 }
 
-// The parts of the items that several shares had, added up in the order of the shares; zeros where a row block saw nothing.
-// A CTA per item.
-template <typename T, int D, int RT>
-__global__ void __launch_bounds__(128) cache_combine_kernel(const CacheAttnParams p) {
+// The parts of the items that several shares had, added up in the order of the shares: a CTA per share, for the item that begins
+// at its end.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) cache_combine_kernel(const CacheAttnParams p) {
   griddep_wait();
   griddep_launch_dependents();
-  const int lane = threadIdx.x & 31;
-  const int items = p.cache.Hk * p.row_blocks;
-  const int b = (int)(blockIdx.x / (unsigned)items), item = (int)(blockIdx.x % (unsigned)items);
-  const int hk = item / p.row_blocks, r0 = (item % p.row_blocks) * RT;
-  bool bad = false;
-  const Span span = span_of(p, b, &bad);
-  if (span.nt == 0) {
-    for (int x = threadIdx.x; x < RT * (D / 4); x += 128)
-      store_row<T>(p, b, hk, r0 + x / (D / 4), (x % (D / 4)) * 4, make_float4(0.f, 0.f, 0.f, 0.f), 0.f, 0.f);
-    return;
-  }
-  // tiles of the list before this item, and in all
-  long long before = 0, total = 0;
-  for (int b0 = 0; b0 < p.batch.B; b0 += 32) {
-    const long long n = b0 + lane < p.batch.B ? (long long)span_of(p, b0 + lane, &bad).nt * items : 0;
-    long long all = n, less = b0 + lane < b ? n : 0;
-#pragma unroll
-    for (int s = 16; s > 0; s >>= 1) {
-      all += __shfl_xor_sync(0xffffffffu, all, s);
-      less += __shfl_xor_sync(0xffffffffu, less, s);
-    }
-    total += all;
-    before += less;
-  }
-  before += (long long)item * span.nt;
-  const Shares sh = make_shares(p, total);
-  auto share_of = [&](long long tile) {  // the share that has it
-    int c = (int)(((tile + 1) * sh.shares - 1) / total);
-    while (sh.begin(c + 1) <= tile) ++c;
-    while (sh.begin(c) > tile) --c;
-    return c;
-  };
-  const int c0 = share_of(before), c1 = share_of(before + span.nt - 1);
-  if (c0 == c1) return;  // one share had all of it
-  for (int x = threadIdx.x; x < RT * (D / 4); x += 128) {
+  const int c0 = blockIdx.x;
+  const int4 head = *part_header(p, c0);
+  const int c1 = head.w;
+  if (c1 <= c0) return;
+  const int hk = head.y / p.row_blocks, r0 = (head.y % p.row_blocks) * RT;
+  for (int x = threadIdx.x; x < RT * (D / 4); x += 256) {
     const int row = x / (D / 4), d = (x % (D / 4)) * 4;
-    float top = FAWS_NEG_INF;
-    for (int c = c0; c <= c1; ++c) top = fmaxf(top, part_slot<D, RT>(p.parts, c, c == c0 ? 1 : 0)[row * (D + 2) + D]);
     float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-    float den = 0.f;
-    for (int c = c0; c <= c1; ++c) {
-      const float* part = part_slot<D, RT>(p.parts, c, c == c0 ? 1 : 0) + row * (D + 2);
-      const float e = part[D] == FAWS_NEG_INF ? 0.f : fast_exp2(part[D] - top);
-      den = fmaf(e, part[D + 1], den);
-      sum.x = fmaf(e, part[d], sum.x); sum.y = fmaf(e, part[d + 1], sum.y);
-      sum.z = fmaf(e, part[d + 2], sum.z); sum.w = fmaf(e, part[d + 3], sum.w);
+    float top = FAWS_NEG_INF, den = 0.f;
+    for (int c = c0; c <= c1; c += 4) {
+      float4 v[4];
+      float2 ml[4];
+      float most = top;
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        ml[y] = make_float2(FAWS_NEG_INF, 0.f);
+        v[y] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (c + y <= c1) {
+          const float* part = part_slot<D>(p, c + y, c + y == c0 ? 1 : 0) + row * (D + 4);
+          v[y] = *reinterpret_cast<const float4*>(part + d);
+          ml[y] = *reinterpret_cast<const float2*>(part + D);
+        }
+        most = fmaxf(most, ml[y].x);
+      }
+      const float keep = top == FAWS_NEG_INF ? 0.f : fast_exp2(top - most);
+      den *= keep;
+      sum.x *= keep; sum.y *= keep; sum.z *= keep; sum.w *= keep;
+      top = most;
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        const float e = ml[y].x == FAWS_NEG_INF ? 0.f : fast_exp2(ml[y].x - most);
+        den = fmaf(e, ml[y].y, den);
+        sum.x = fmaf(e, v[y].x, sum.x); sum.y = fmaf(e, v[y].y, sum.y);
+        sum.z = fmaf(e, v[y].z, sum.z); sum.w = fmaf(e, v[y].w, sum.w);
+      }
     }
-    store_row<T>(p, b, hk, r0 + row, d, sum, top, den);
+    store_row<T>(p, head.x, hk, r0 + row, d, sum, top, den);
   }
 }
 
@@ -1010,20 +1037,14 @@ cudaError_t launch_overlapped(K kernel, dim3 grid, int threads, size_t smem, cud
   return e != cudaSuccess ? e : cudaGetLastError();
 }
 
-template <typename T, int D, int RT>
-cudaError_t launch_attn_r(CacheAttnParams p, cudaStream_t s) {
-  using L = CacheSmem<D, RT>;
-  static PerDeviceOnce once;
-  if (cudaError_t e = set_max_smem_once(once, cache_attn_kernel<T, D, RT>, L::total); e != cudaSuccess) return e;
-  p.row_blocks = (p.rows + RT - 1) / RT;
-  if (cudaError_t e = launch_overlapped(cache_attn_kernel<T, D, RT>, dim3(p.grid), CTA_THREADS, L::total, s, p); e != cudaSuccess)
-    return e;
-  const unsigned items = (unsigned)(p.batch.B * p.cache.Hk * p.row_blocks);
-  return launch_overlapped(cache_combine_kernel<T, D, RT>, dim3(items), 128, 0, s, p);
-}
 template <typename T, int D>
-cudaError_t launch_attn_d(const CacheAttnParams& p, cudaStream_t s) {
-  return p.rows <= 8 ? launch_attn_r<T, D, 8>(p, s) : launch_attn_r<T, D, 16>(p, s);
+cudaError_t launch_attn_d(CacheAttnParams p, cudaStream_t s) {
+  static PerDeviceOnce once;
+  if (cudaError_t e = set_max_smem_once(once, cache_attn_kernel<T, D>, CacheSmem<D>::total); e != cudaSuccess) return e;
+  p.row_blocks = (p.rows + RT - 1) / RT;
+  if (cudaError_t e = launch_overlapped(cache_attn_kernel<T, D>, dim3(p.grid), CTA_THREADS, CacheSmem<D>::total, s, p); e != cudaSuccess)
+    return e;
+  return launch_overlapped(cache_combine_kernel<T, D>, dim3(p.grid), 256, 0, s, p);
 }
 template <typename T>
 cudaError_t launch_attn_t(const CacheAttnParams& p, cudaStream_t s) {
@@ -1035,7 +1056,7 @@ cudaError_t launch_attn_t(const CacheAttnParams& p, cudaStream_t s) {
   }
 }
 
-int shares_at_most(int rows) { return ctas_per_sm(rows <= 8 ? 8 : 16) * sm_count(); }
+int shares_at_most() { return CTAS_PER_SM * sm_count(); }
 
 template <typename T, bool WRITE, int D>
 cudaError_t launch_rows_d(const CacheParams& c, const CacheBatch& b, CacheRows r, cudaStream_t s) {
@@ -1087,14 +1108,12 @@ cudaError_t launch_cache_read(const CacheParams& c, const CacheBatch& b, const f
   return dtype == FAWS_FP16 ? launch_rows_t<__half, false>(c, b, r, s) : launch_rows_t<__nv_bfloat16, false>(c, b, r, s);
 }
 
-size_t cache_attn_workspace_bytes(int rows, int D) {
-  return (size_t)shares_at_most(rows) * 2 * (rows <= 8 ? 8 : 16) * (D + 2) * 4;
-}
+size_t cache_attn_workspace_bytes(int D) { return (size_t)shares_at_most() * (16 + 2 * RT * (D + 4) * 4); }
 
 cudaError_t launch_cache_attn(const CacheAttnParams& call, int dtype, cudaStream_t s) {
   CacheAttnParams p = call;
-  p.grid = shares_at_most(p.rows);
-  p.min_tiles = 2;
+  p.grid = shares_at_most();
+  p.min_tiles = 1;
   p.vec_out = reinterpret_cast<uintptr_t>(p.out) % 8 == 0 && p.o_sb % 4 == 0 && p.o_sh % 4 == 0 && p.o_ss % 4 == 0;
   p.status = tc_status_word();
   return dtype == FAWS_FP16 ? launch_attn_t<__half>(p, s) : launch_attn_t<__nv_bfloat16>(p, s);

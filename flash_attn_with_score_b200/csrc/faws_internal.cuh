@@ -240,7 +240,7 @@ cudaError_t launch_cache_write(const CacheParams& c, const CacheBatch& b, const 
                                int dtype, cudaStream_t s);
 cudaError_t launch_cache_read(const CacheParams& c, const CacheBatch& b, const faws_tensor* k, const faws_tensor* v, int rows,
                               int dtype, cudaStream_t s);
-size_t cache_attn_workspace_bytes(int rows, int D);
+size_t cache_attn_workspace_bytes(int D);
 cudaError_t launch_cache_attn(const CacheAttnParams& p, int dtype, cudaStream_t s);  // p.parts = the workspace
 cudaError_t launch_generic_scores_only(const ScoresOnlyParams& p, int dtype, cudaStream_t s);
 bool tc_scores_only_supported(const ScoresOnlyParams& p, int dtype);
