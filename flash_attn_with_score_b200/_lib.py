@@ -139,18 +139,29 @@ OP_SCORES_ONLY = 100  # of plain_call alone: compute_attention_scores has no wor
 _plain = None  # the native call once it is imported, False where it cannot be
 
 
+def _import_plain():
+    global _plain
+    try:
+        from . import _plain as module
+        _plain = module.call
+    except ImportError:
+        _plain = False
+
+
 def plain_call(*args):
     """Runs ``(op, q, k, v, causal, sm_scale, split, per_q_head)`` natively, outputs and launch, or returns None where a
     tensor or the moment is out of the ordinary (csrc/faws_torch.cpp), or _plain.so is missing or was built for another
     torch or Python: the caller then goes the long way."""
-    global _plain
     if _plain is None:
-        try:
-            from . import _plain as module
-            _plain = module.call
-        except ImportError:
-            _plain = False
+        _import_plain()
     return _plain(*args) if _plain else None
+
+
+def plain(name, *args):
+    """The same for the operators with a native call of their own: ``window``, ``cache_write``, ``cache_read``, ``cache_attention``."""
+    if _plain is None:
+        _import_plain()
+    return getattr(_plain.__self__, name)(*args) if _plain else None
 
 
 def check(status: int, what: str):

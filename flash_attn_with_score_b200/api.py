@@ -284,6 +284,10 @@ def attention_with_window(q, k, v, window, sinks=0, sm_scale=None, return_log_no
     window, sinks = min(int(window), _NO_LIMIT), min(int(sinks), _NO_LIMIT)
     assert window >= 1, "window must be at least 1"
     assert sinks >= 0, "sinks must not be negative"
+    if backend is None and kv_splits is None:
+        got = _lib.plain("window", q, k, v, window, sinks, sm_scale, return_log_normalizer)
+        if got is not None:
+            return got
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         out, L = _WindowFunction.apply(q, k, v, window, sinks, sm_scale, backend, kv_splits)
     else:

@@ -17,7 +17,7 @@ import math
 import torch
 
 from . import _lib
-from .api import _DTYPES, _raw_stream, _tensor, maybe_contiguous
+from .api import _DTYPES, _NO_LIMIT, _raw_stream, _tensor, maybe_contiguous
 
 
 class KVCache4:
@@ -46,6 +46,7 @@ class KVCache4:
             raise RuntimeError("flash_attn_with_score_b200 runs on CUDA tensors only (no CPU fallback)")
         self._struct = _lib.KVCache(self.k_codes.data_ptr(), self.v_codes.data_ptr(), self.k_scales.data_ptr(),
                                     self.v_scales.data_ptr(), pages, page_size, heads, head_dim, _DTYPES[dtype])
+        self._plain = (C.addressof(self._struct), self.device.index)
 
 
 def _batch(cache, page_table, lengths, B):
@@ -75,6 +76,8 @@ def _run(cache, name, *args):
 def kv_cache_write(cache, k, v, page_table, lengths):
     """Quantises k and v (B, Hk, M, D), the last M rows of each sequence, into the cache; padding rows are skipped.  Rows of one
     call are to go to different places (a page that several sequences share may be read by all, written by none)."""
+    if type(cache) is KVCache4 and _lib.plain("cache_write", *cache._plain, k, v, page_table, lengths):
+        return
     assert k.dim() == 4 and k.shape == v.shape, "k and v must have the same (B, Hk, M, D)"
     B, Hk, M, D = k.shape
     table, lens, batch = _batch(cache, page_table, lengths, B)
@@ -91,6 +94,10 @@ def kv_cache_write(cache, k, v, page_table, lengths):
 def kv_cache_read(cache, page_table, lengths, rows):
     """``(k, v)``, each (B, Hk, rows, D) in the cache's dtype: the values that the cache holds of the last ``rows`` positions of each
     sequence, zeros in padding rows."""
+    if type(cache) is KVCache4:
+        got = _lib.plain("cache_read", *cache._plain, page_table, lengths, rows)
+        if got is not None:
+            return got
     B = lengths.shape[0]
     table, lens, batch = _batch(cache, page_table, lengths, B)
     assert rows >= 0, "rows must not be negative"
@@ -108,13 +115,18 @@ def attention_with_kv_cache(q, cache, page_table, lengths, window=None, sinks=0,
     A row sees the keys up to its own position; with ``window`` the last ``window`` of them (its own among them) and the
     first ``sinks`` of the sequence.  Rows that see nothing (padding, empty sequences) become 0, their log-normaliser -inf.
     Returns ``out`` (B, Hq, M, D), or ``(out, log_normalizer)``, the latter (B, Hq, M) fp32.  Forward only; any M, made for few rows."""
+    assert window is None or window >= 1, "window must be at least 1"
+    assert sinks >= 0, "sinks must not be negative"
+    window, sinks = min(int(window), _NO_LIMIT) if window is not None else 0, min(int(sinks), _NO_LIMIT)
+    if type(cache) is KVCache4:
+        got = _lib.plain("cache_attention", *cache._plain, q, page_table, lengths, window, sinks, sm_scale, return_log_normalizer)
+        if got is not None:
+            return got
     assert q.dim() == 4, "q must be (B, Hq, M, D)"
     B, H, M, D = q.shape
     table, lens, batch = _batch(cache, page_table, lengths, B)
     assert D == cache.head_dim, f"feature size of q is {D}, the cache's {cache.head_dim}"
     assert H > 0 and H % cache.heads == 0, "number of heads in q must be a multiple of that in the cache"
-    assert window is None or window >= 1, "window must be at least 1"
-    assert sinks >= 0, "sinks must not be negative"
     if q.dtype != cache.dtype:
         raise TypeError(f"q must be {cache.dtype} as the cache is, got {q.dtype}")
     assert q.device == cache.device, "q must be on the cache's device"
@@ -130,5 +142,5 @@ def attention_with_kv_cache(q, cache, page_table, lengths, window=None, sinks=0,
         n = _lib.load().faws_kv_cache_workspace_bytes(C.byref(p))
         ws = torch.empty(n, device=q.device, dtype=torch.uint8)
         _run(cache, "faws_attention_with_kv_cache", C.byref(p), C.byref(cache._struct), C.byref(batch),
-             min(int(window), 2 ** 31 - 1) if window is not None else 0, min(int(sinks), 2 ** 31 - 1), C.c_void_p(ws.data_ptr()), n)
+             window, sinks, C.c_void_p(ws.data_ptr()), n)
     return (out, L) if return_log_normalizer else out
