@@ -694,7 +694,7 @@ tc_fwd_kernel(const __grid_constant__ TcMaps maps, const FwdParams p, const __gr
       // S512 D64 10.6 -> 11.6), nor under column sums, whose shuffles would; nor with 128-row CTAs, few of whose tiles are not
       // masked and whose chain it lengthens (fp16 B10 H16
       // M34 N617 D128 causal 20.6 us, 20.0 without).
-      constexpr bool kRolled = kMasked && (!SPLIT || WIN) && (HOOK == kHookNone || HOOK == kHookRowSum);
+      constexpr bool kRolled = kMasked && !SPLIT && !WIN && (HOOK == kHookNone || HOOK == kHookRowSum);
       constexpr bool kDraw = DROP == kDrawMask || DROP == kKeepMask;
       constexpr bool kReread = kRolled || (kDraw && HOOK == kHookNone);
       uint32_t r[kRolled ? 1 : 128];
@@ -704,18 +704,22 @@ tc_fwd_kernel(const __grid_constant__ TcMaps maps, const FwdParams p, const __gr
         if (p.causal) lim = min(lim, FEW || WIN ? vis_end : i + p.p_seq + 1);
         nvis = max(0, min(128, lim - n0));
       }
-      // WIN: the window's keys of the row are columns [xlo, nvis), the sinks those before xsink
-      [[maybe_unused]] int xlo = 0, xsink = 0;
+      // WIN: the window's keys of the row are columns [xlo, nvis), the sinks those before xsink.  Bit x of vis_word[c]: the row
+      // sees column 32 c + x; bit c of live: some row of the warp sees one of the 32.  Chunks that none sees are not
+      // exponentiated: of the 16 of a query tile a window's first and last key tile have ten, a tile of a few sinks four.
+      [[maybe_unused]] uint32_t vis_word[4] = {0u, 0u, 0u, 0u};
+      [[maybe_unused]] int live = 0xf;
       if constexpr (kMasked && WIN) {
-        xlo = vis_end - p.window - n0;
-        xsink = p.sinks - n0;
-      }
-      // bit x: the row sees column 32 c + x
-      [[maybe_unused]] auto visible_word = [&](int c) -> uint32_t {
         auto below = [](int n) -> uint32_t { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u; };
-        return below(nvis - c * 32) & (~below(xlo - c * 32) | below(xsink - c * 32));
-      };
-#define FAWS_VIS(x) (!kMasked || (x) < nvis)
+        const int xlo = vis_end - p.window - n0, xsink = p.sinks - n0;
+        live = 0;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          vis_word[c] = below(nvis - c * 32) & (~below(xlo - c * 32) | below(xsink - c * 32));
+          live |= __any_sync(0xffffffffu, vis_word[c] != 0u) ? 1 << c : 0;
+        }
+      }
+#define FAWS_VIS(x) (!kMasked || (WIN ? (vis_word[(x) >> 5] >> ((x) & 31) & 1u) != 0u : (x) < nvis))
 
       // ---- row max (4 independent chains)
       float a0 = FAWS_NEG_INF, a1 = FAWS_NEG_INF, a2 = FAWS_NEG_INF, a3 = FAWS_NEG_INF;
@@ -723,11 +727,6 @@ tc_fwd_kernel(const __grid_constant__ TcMaps maps, const FwdParams p, const __gr
         [[maybe_unused]] float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
 #pragma unroll 1
         for (int c = 0; c < 4; ++c) {
-          [[maybe_unused]] uint32_t word = 0u;
-          if constexpr (WIN) {
-            word = visible_word(c);
-            if (!__any_sync(0xffffffffu, word != 0u)) continue;
-          }
           uint32_t sv[32];
           tmem_ld32(t_s + c * 32, sv);
           tmem_wait_ld();
@@ -736,8 +735,7 @@ tc_fwd_kernel(const __grid_constant__ TcMaps maps, const FwdParams p, const __gr
           for (int x = 0; x < 32; x += 8) {
             float y[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-              y[e] = (WIN ? (word >> (x + e) & 1u) != 0u : x + e < nv) ? __uint_as_float(sv[x + e]) : FAWS_NEG_INF;
+            for (int e = 0; e < 8; ++e) y[e] = x + e < nv ? __uint_as_float(sv[x + e]) : FAWS_NEG_INF;
             a0 = fmax3(a0, y[0], y[1]);
             a1 = fmax3(a1, y[2], y[3]);
             a2 = fmax3(a2, y[4], y[5]);
@@ -761,6 +759,7 @@ tc_fwd_kernel(const __grid_constant__ TcMaps maps, const FwdParams p, const __gr
 #define FAWS_SV(x) (FAWS_VIS(x) ? __uint_as_float(r[x]) : FAWS_NEG_INF)
 #pragma unroll
         for (int x = 0; x < 128; x += 8) {  // three-input max: 64 instructions for 128 values
+          if (kMasked && WIN && !(live >> (x >> 5) & 1)) continue;
           a0 = fmax3(a0, FAWS_SV(x), FAWS_SV(x + 1));
           a1 = fmax3(a1, FAWS_SV(x + 2), FAWS_SV(x + 3));
           a2 = fmax3(a2, FAWS_SV(x + 4), FAWS_SV(x + 5));
@@ -805,8 +804,7 @@ tc_fwd_kernel(const __grid_constant__ TcMaps maps, const FwdParams p, const __gr
       auto p_chunk = [&](int c, const uint32_t (&sv)[32]) {  // 32 key columns
         uint32_t pk[16];
         [[maybe_unused]] uint32_t bits = 0u;  // kKeepMask (zero where the warp's rows see nothing: such weights are zero)
-        [[maybe_unused]] const uint32_t word = kMasked && WIN ? visible_word(c) : 0u;
-        const bool block_hidden = kMasked && (WIN ? !__any_sync(0xffffffffu, word != 0u) : c * 32 >= nvis_warp);
+        const bool block_hidden = kMasked && (WIN ? !(live >> c & 1) : c * 32 >= nvis_warp);
         if (block_hidden) {
 #pragma unroll
           for (int x = 0; x < 16; ++x) pk[x] = 0u;
@@ -824,13 +822,8 @@ tc_fwd_kernel(const __grid_constant__ TcMaps maps, const FwdParams p, const __gr
             unpack_f32x2(t2, t0, t1);
             t0 = fast_exp2(t0);
             t1 = fast_exp2(t1);
-            if constexpr (kMasked && WIN) {
-              e[y] = word >> (g * 8 + y) & 1u ? t0 : 0.f;
-              e[y + 1] = word >> (g * 8 + y + 1) & 1u ? t1 : 0.f;
-            } else {
-              e[y] = FAWS_VIS(x) ? t0 : 0.f;
-              e[y + 1] = FAWS_VIS(x + 1) ? t1 : 0.f;
-            }
+            e[y] = FAWS_VIS(x) ? t0 : 0.f;
+            e[y + 1] = FAWS_VIS(x + 1) ? t1 : 0.f;
           }
           lp0 = add_f32x2(lp0, add_f32x2(pack_f32x2(e[0], e[1]), pack_f32x2(e[4], e[5])));
           lp1 = add_f32x2(lp1, add_f32x2(pack_f32x2(e[2], e[3]), pack_f32x2(e[6], e[7])));
@@ -1393,7 +1386,7 @@ cudaError_t launch_fwd_s(const TcMaps& maps, const FwdParams& p, cudaStream_t s)
   FwdParams pp = p;
   // K and V of all heads together stay resident in the 126 MB L2 -> order CTAs for load balance
   const long long kv_bytes = 2LL * p.B * p.Hk * p.N * p.D * 2;
-  pp.lpt_order = (!WIN && p.causal && kv_bytes <= (48LL << 20) && 2 * ncb <= 65535) ? 1 : 0;
+  pp.lpt_order = (p.causal && kv_bytes <= (48LL << 20) && 2 * ncb <= 65535) ? 1 : 0;
   // masked key tiles exist (causal, some row block ends before N): give them their own CTAs
   pp.fill_ctas = ((HOOK == kHookScores || HOOK == kHookScores16 || HOOK == kHookScoresAny) && p.causal &&
                    p.p_seq + std::min(p.m_begin + BM, p.m_end) < p.N) ? 1 : 0;
