@@ -62,9 +62,13 @@ template <typename T> __device__ __forceinline__ uint32_t code_times_scale(uint3
 template <> __device__ __forceinline__ uint32_t code_times_scale<__half>(uint32_t nibbles, uint32_t scale) {
   nibbles |= 0x64006400u;  // 1024 + n
   const __half2 c = __hsub2(*reinterpret_cast<__half2*>(&nibbles), __floats2half2_rn(1032.f, 1032.f));
+  const float sf = __uint_as_float(scale << 16);
+  if (scale >= 0x3780u) {  // from 2^-16 on a bf16 number is an fp16 one (of a group of fp16 numbers: at most 2^13.2), or NaN
+    const __half2 v = __hmul2(c, __float2half2_rn(sf));
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
   const float2 f = __half22float2(c);
-  const float s = __uint_as_float(scale << 16);  // (may be smaller than fp16 holds exactly)
-  const __half2 v = __floats2half2_rn(f.x * s, f.y * s);
+  const __half2 v = __floats2half2_rn(f.x * sf, f.y * sf);
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 template <> __device__ __forceinline__ uint32_t code_times_scale<__nv_bfloat16>(uint32_t nibbles, uint32_t scale) {
@@ -95,7 +99,8 @@ __device__ __forceinline__ int cached_length(const CacheBatch& c, int page_shift
 // ---------------------------------------------------------------------------------------------- write, read
 // A thread has 8 neighbouring elements of a row; TPR = D / 8 threads a row, the four (D 16: two) of a group next to each other.
 // Bound by HBM: 2 bytes read and 9/16 written an element (reading back: the other way round).  A CTA takes consecutive rows
-// of one sequence and head, a thread kRowsEach of them, so that what a row costs beside its elements is little.
+// of one sequence and head, a thread four of them, so that what a row costs beside its elements is little, or one where a
+// sequence has no more than a CTA's.
 struct CacheRows {
   const void* src[2];  // write: k, v; read: unused
   void* dst[2];        // read: k, v
@@ -106,14 +111,37 @@ struct CacheRows {
 };
 constexpr int kRowsEach = 4;
 
-// Row of the cache's tensors that holds position pos; -1 for a page that does not exist.
-__device__ __forceinline__ int64_t cache_row(const CacheParams& c, const int32_t* table, int hk, int pos, bool* bad) {
-  const int page = table[pos >> c.page_shift];
-  if ((unsigned)page >= (unsigned)c.pages) {
-    *bad = true;
-    return -1;
+// What the rows of a CTA have in common, and where row m of its sequence and head lies in the cache's tensors (-1: on a page that
+// does not exist).  The CTA's rows mostly lie on one page, which is then looked up once.
+struct RowPlace {
+  const int32_t* table;
+  int first;           // position of row 0
+  int shift, pages, Hk, hk;
+  int one;             // the page of all rows, or kSeveral
+  static constexpr int kSeveral = -0x7fffffff;
+  __device__ __forceinline__ bool real(int m, int rows) const { return m < rows && first + m >= 0; }
+  __device__ __forceinline__ int64_t at(int m, bool* bad) const {
+    const int pos = first + m, page = one != kSeveral ? one : table[pos >> shift];
+    if ((unsigned)page >= (unsigned)pages) {
+      *bad = true;
+      return -1;
+    }
+    return (((int64_t)page * Hk + hk) << shift) + (pos & ((1 << shift) - 1));
   }
-  return (((int64_t)page * c.Hk + hk) << c.page_shift) + (pos & ((1 << c.page_shift) - 1));
+};
+// of the CTA's rows [m0, m1)
+__device__ __forceinline__ RowPlace row_place(const CacheParams& c, const CacheBatch& bt, int rows, int b, int hk, int m0, int m1,
+                                              bool* bad) {
+  RowPlace p;
+  p.table = bt.table + (int64_t)b * bt.table_stride;
+  p.first = cached_length(bt, c.page_shift, b, bad) - rows;
+  p.shift = c.page_shift;
+  p.pages = c.pages;
+  p.Hk = c.Hk;
+  p.hk = hk;
+  const int lo = max(p.first + m0, 0) >> c.page_shift, hi = (p.first + min(m1, rows) - 1) >> c.page_shift;
+  p.one = lo == hi ? p.table[lo] : RowPlace::kSeveral;  // (hi < 0: no row is real)
+  return p;
 }
 
 // The words of a row of values as they lie in memory, from the words of elements (`to` true), or back.  Word p of the row: half-words
@@ -137,42 +165,39 @@ __device__ __forceinline__ uint32_t exchange_halves(uint32_t word, int w, bool t
 __device__ __forceinline__ uint32_t rotate_halves(uint32_t x) { return (x << 2 & 0xfffcfffcu) | (x >> 14 & 0x00030003u); }
 __device__ __forceinline__ uint32_t rotate_halves_back(uint32_t x) { return (x >> 2 & 0x3fff3fffu) | (x << 14 & 0xc000c000u); }
 
-template <typename T, int D>
-__global__ void __launch_bounds__(256) cache_write_kernel(CacheParams c, CacheBatch bt, CacheRows r, int* status) {
+// A CTA's rows: `lanes` at a time from row `first` of sequence b and head hk on.
+struct RowTile {
+  int b, hk, first, lanes;
+};
+
+template <typename T, int D, bool VALUES, bool WHOLE, int EACH>
+__device__ __forceinline__ void write_rows(const CacheParams& c, const CacheRows& r, const RowPlace& place, const RowTile& t, bool* bad) {
   constexpr int TPR = D / 8, NG = D >= 32 ? D / 32 : 1, GL = D >= 32 ? 4 : 2;
   constexpr uint32_t kInfinity = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
-  griddep_wait();
-  griddep_launch_dependents();
-  const int w = threadIdx.x % TPR, lanes = blockDim.x / TPR;
-  const int bh = blockIdx.x / (unsigned)r.tiles, tile = blockIdx.x - bh * r.tiles;
-  const int b = bh / (unsigned)c.Hk, hk = bh - b * c.Hk;
-  const bool second = blockIdx.y != 0;
-  bool bad = false;
-  const int first = cached_length(bt, c.page_shift, b, &bad) - r.rows;  // position of row 0
-  const int32_t* table = bt.table + (int64_t)b * bt.table_stride;
-  const T* src = static_cast<const T*>(second ? r.src[1] : r.src[0]) + b * (second ? r.sb[1] : r.sb[0]) +
-                 hk * (second ? r.sh[1] : r.sh[0]) + w * 8;
-  const int64_t ss = second ? r.ss[1] : r.ss[0];
-  unsigned char* codes = static_cast<unsigned char*>(second ? c.v_codes : c.k_codes);
-  uint16_t* scales = static_cast<uint16_t*>(second ? c.v_scales : c.k_scales);
-  const int m0 = tile * lanes * kRowsEach + threadIdx.x / TPR;
-  uint4 in[kRowsEach];
+  const int w = threadIdx.x % TPR, lanes = t.lanes, m0 = t.first + threadIdx.x / TPR;
+  // WHOLE: the rows lie one behind the other
+  const int64_t row0 = WHOLE ? place.at(m0, bad) : 0;
+  const int64_t ss = r.ss[VALUES];
+  const T* src = static_cast<const T*>(r.src[VALUES]) + t.b * r.sb[VALUES] + t.hk * r.sh[VALUES] + m0 * ss + w * 8;
+  unsigned char* codes = static_cast<unsigned char*>(VALUES ? c.v_codes : c.k_codes) + (D >= 32 && !VALUES ? (w % 4) * NG + w / 4 : w) * 4;
+  uint16_t* scales = static_cast<uint16_t*>(VALUES ? c.v_scales : c.k_scales) + w / GL;
+  uint4 in[EACH];
 #pragma unroll
-  for (int y = 0; y < kRowsEach; ++y) {
-    const int m = m0 + y * lanes;
+  for (int y = 0; y < EACH; ++y) {
     in[y] = make_uint4(0u, 0u, 0u, 0u);
-    if (m < r.rows && first + m >= 0) {
-      if (r.vec) in[y] = *reinterpret_cast<const uint4*>(src + m * ss);
+    if (WHOLE || place.real(m0 + y * lanes, r.rows)) {
+      const T* from = src + y * lanes * ss;
+      if (WHOLE || r.vec) in[y] = *reinterpret_cast<const uint4*>(from);
       else {
         uint16_t e[8];
 #pragma unroll
-        for (int x = 0; x < 8; ++x) e[x] = reinterpret_cast<const uint16_t*>(src + m * ss)[x];
+        for (int x = 0; x < 8; ++x) e[x] = reinterpret_cast<const uint16_t*>(from)[x];
         in[y] = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
       }
     }
   }
 #pragma unroll
-  for (int y = 0; y < kRowsEach; ++y) {
+  for (int y = 0; y < EACH; ++y) {
     const int m = m0 + y * lanes;
     const uint32_t v[4] = {in[y].x, in[y].y, in[y].z, in[y].w};
     // largest magnitude of the group, as integers, as which they order alike; infinities and NaN come last
@@ -203,72 +228,92 @@ __global__ void __launch_bounds__(256) cache_write_kernel(CacheParams c, CacheBa
 #pragma unroll
     for (int e = 6; e >= 0; --e) word = word * 16u + __float_as_uint(fmaf(x[e], inv, 8388616.f));
     word -= 0xfb000000u;  // what is left of 2^23, 0x4b000000 in elements 0 and 1
-    if (D >= 32) word = second ? exchange_halves<D>(rotate_halves(word), w, true) : __funnelshift_l(word, word, 2);
-    if (m < r.rows && first + m >= 0) {
-      const int64_t row = cache_row(c, table, hk, first + m, &bad);
-      if (row >= 0) {
-        const int at = D >= 32 && !second ? (w % 4) * NG + w / 4 : w;
-        *reinterpret_cast<uint32_t*>(codes + row * (D / 2) + at * 4) = word;
-        if (w % GL == 0) scales[row * NG + w / GL] = (uint16_t)sbits;
+    if (D >= 32) word = VALUES ? exchange_halves<D>(rotate_halves(word), w, true) : __funnelshift_l(word, word, 2);
+    if (WHOLE || place.real(m, r.rows)) {
+      const int64_t row = WHOLE ? row0 + y * lanes : place.at(m, bad);
+      if (WHOLE || row >= 0) {
+        *reinterpret_cast<uint32_t*>(codes + row * (D / 2)) = word;
+        if (w % GL == 0) scales[row * NG] = (uint16_t)sbits;
       }
     }
   }
-  if (bad && status != nullptr) atomicOr(status, kBadPage);
 }
 
-template <typename T, int D>
-__global__ void __launch_bounds__(256) cache_read_kernel(CacheParams c, CacheBatch bt, CacheRows r, int* status) {
+template <typename T, int D, bool VALUES, bool WHOLE, int EACH>
+__device__ __forceinline__ void read_rows(const CacheParams& c, const CacheRows& r, const RowPlace& place, const RowTile& t, bool* bad) {
   constexpr int TPR = D / 8, NG = D >= 32 ? D / 32 : 1, GL = D >= 32 ? 4 : 2;
-  griddep_wait();
-  griddep_launch_dependents();
-  const int w = threadIdx.x % TPR, lanes = blockDim.x / TPR;
-  const int bh = blockIdx.x / (unsigned)r.tiles, tile = blockIdx.x - bh * r.tiles;
-  const int b = bh / (unsigned)c.Hk, hk = bh - b * c.Hk;
-  const bool second = blockIdx.y != 0;
-  bool bad = false;
-  const int first = cached_length(bt, c.page_shift, b, &bad) - r.rows;
-  const int32_t* table = bt.table + (int64_t)b * bt.table_stride;
-  const unsigned char* codes = static_cast<const unsigned char*>(second ? c.v_codes : c.k_codes);
-  const uint16_t* scales = static_cast<const uint16_t*>(second ? c.v_scales : c.k_scales);
-  const int m0 = tile * lanes * kRowsEach + threadIdx.x / TPR;
-  const int at = D >= 32 && !second ? (w % 4) * NG + w / 4 : w;
-  uint32_t words[kRowsEach], sbits[kRowsEach];
+  const int w = threadIdx.x % TPR, lanes = t.lanes, m0 = t.first + threadIdx.x / TPR;
+  // WHOLE: the rows lie one behind the other
+  const int64_t row0 = WHOLE ? place.at(m0, bad) : 0;
+  const unsigned char* codes =
+      static_cast<const unsigned char*>(VALUES ? c.v_codes : c.k_codes) + (D >= 32 && !VALUES ? (w % 4) * NG + w / 4 : w) * 4;
+  const uint16_t* scales = static_cast<const uint16_t*>(VALUES ? c.v_scales : c.k_scales) + w / GL;
+  uint32_t words[EACH], sbits[EACH];
 #pragma unroll
-  for (int y = 0; y < kRowsEach; ++y) {
+  for (int y = 0; y < EACH; ++y) {
     const int m = m0 + y * lanes;
     words[y] = D >= 32 ? 0x22222222u : 0x88888888u;  // padding: zeros
     sbits[y] = 0u;
-    if (m < r.rows && first + m >= 0) {
-      const int64_t row = cache_row(c, table, hk, first + m, &bad);
+    if (WHOLE || place.real(m, r.rows)) {
+      const int64_t row = WHOLE ? row0 + y * lanes : place.at(m, bad);
       sbits[y] = 0xffc0u;
-      if (row >= 0) {
-        words[y] = *reinterpret_cast<const uint32_t*>(codes + row * (D / 2) + at * 4);
-        sbits[y] = scales[row * NG + w / GL];
+      if (WHOLE || row >= 0) {
+        words[y] = *reinterpret_cast<const uint32_t*>(codes + row * (D / 2));
+        sbits[y] = scales[row * NG];
       }
     }
   }
-  T* dst = static_cast<T*>(second ? r.dst[1] : r.dst[0]) + b * (second ? r.sb[1] : r.sb[0]) +
-           hk * (second ? r.sh[1] : r.sh[0]) + w * 8;
-  const int64_t ss = second ? r.ss[1] : r.ss[0];
+  const int64_t ss = r.ss[VALUES];
+  T* dst = static_cast<T*>(r.dst[VALUES]) + t.b * r.sb[VALUES] + t.hk * r.sh[VALUES] + m0 * ss + w * 8;
 #pragma unroll
-  for (int y = 0; y < kRowsEach; ++y) {
-    const int m = m0 + y * lanes;
+  for (int y = 0; y < EACH; ++y) {
     uint32_t word = words[y];
-    if (D >= 32) word = second ? rotate_halves_back(exchange_halves<D>(word, w, false)) : __funnelshift_r(word, word, 2);
+    if (D >= 32) word = VALUES ? rotate_halves_back(exchange_halves<D>(word, w, false)) : __funnelshift_r(word, word, 2);
     // elements (0, 4), (1, 5), (2, 6), (3, 7), each exact as a 16-bit number; their products are rounded once
     uint32_t pair[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) pair[e] = code_times_scale<T>(word >> (4 * e) & 0x000f000fu, sbits[y]);
     const uint4 out = make_uint4(__byte_perm(pair[0], pair[1], 0x5410), __byte_perm(pair[2], pair[3], 0x5410),
                                  __byte_perm(pair[0], pair[1], 0x7632), __byte_perm(pair[2], pair[3], 0x7632));
-    if (m < r.rows) {
-      if (r.vec) *reinterpret_cast<uint4*>(dst + m * ss) = out;
+    if (WHOLE || m0 + y * lanes < r.rows) {
+      T* to = dst + y * lanes * ss;
+      if (WHOLE || r.vec) *reinterpret_cast<uint4*>(to) = out;
       else {
         const uint32_t o[4] = {out.x, out.y, out.z, out.w};
 #pragma unroll
-        for (int e = 0; e < 8; ++e) reinterpret_cast<uint16_t*>(dst + m * ss)[e] = (uint16_t)(o[e / 2] >> (16 * (e & 1)));
+        for (int e = 0; e < 8; ++e) reinterpret_cast<uint16_t*>(to)[e] = (uint16_t)(o[e / 2] >> (16 * (e & 1)));
       }
     }
+  }
+}
+
+// Keys in the first half of the grid, values in the second.  CTAs whose rows all exist, on one page, with 16-byte accesses, go
+// without the checks for each row (bf16 and fp16, 4 sequences of 8192 rows of 8 heads of 128: written in 42.7 us and read in 43.7 and
+// 50.8 with them).
+template <typename T, int D, bool WRITE, int EACH>
+__global__ void __launch_bounds__(256) cache_rows_kernel(const CacheParams c, const CacheBatch bt, const CacheRows r, int* status) {
+  griddep_wait();
+  griddep_launch_dependents();
+  RowTile t;
+  const int bh = blockIdx.x / (unsigned)r.tiles;
+  t.b = bh / (unsigned)c.Hk;
+  t.hk = bh - t.b * c.Hk;
+  t.lanes = blockDim.x / (D / 8);
+  const int rows = t.lanes * EACH;
+  t.first = (blockIdx.x - bh * r.tiles) * rows;
+  bool bad = false;
+  const RowPlace place = row_place(c, bt, r.rows, t.b, t.hk, t.first, t.first + rows, &bad);
+  const bool whole = r.vec && t.first + rows <= r.rows && place.first + t.first >= 0 && (unsigned)place.one < (unsigned)c.pages;
+  auto run = [&](auto values, auto all) {
+    if constexpr (WRITE) write_rows<T, D, decltype(values)::value, decltype(all)::value, EACH>(c, r, place, t, &bad);
+    else read_rows<T, D, decltype(values)::value, decltype(all)::value, EACH>(c, r, place, t, &bad);
+  };
+  if (blockIdx.y == 0) {
+    if (whole) run(std::false_type{}, std::true_type{});
+    else run(std::false_type{}, std::false_type{});
+  } else {
+    if (whole) run(std::true_type{}, std::true_type{});
+    else run(std::true_type{}, std::false_type{});
   }
   if (bad && status != nullptr) atomicOr(status, kBadPage);
 }
@@ -1061,12 +1106,13 @@ int shares_at_most() { return CTAS_PER_SM * sm_count(); }
 template <typename T, bool WRITE, int D>
 cudaError_t launch_rows_d(const CacheParams& c, const CacheBatch& b, CacheRows r, cudaStream_t s) {
   // few rows (decoding): small CTAs, so that heads and sequences fill the chip
+  const int each = r.rows * (D / 8) <= 256 ? 1 : kRowsEach;
   int lanes = 32 / (D / 8) > 1 ? 32 / (D / 8) : 1;
-  while (lanes * (D / 8) < 256 && lanes * kRowsEach < r.rows) lanes *= 2;
-  r.tiles = (r.rows + lanes * kRowsEach - 1) / (lanes * kRowsEach);
+  while (lanes * (D / 8) < 256 && lanes * each < r.rows) lanes *= 2;
+  r.tiles = (r.rows + lanes * each - 1) / (lanes * each);
   const dim3 grid((unsigned)((int64_t)b.B * c.Hk * r.tiles), 2, 1);
-  return launch_overlapped(WRITE ? cache_write_kernel<T, D> : cache_read_kernel<T, D>, grid, lanes * (D / 8), 0, s, c, b, r,
-                           tc_status_word());
+  return launch_overlapped(each == 1 ? cache_rows_kernel<T, D, WRITE, 1> : cache_rows_kernel<T, D, WRITE, kRowsEach>, grid,
+                           lanes * (D / 8), 0, s, c, b, r, tc_status_word());
 }
 template <typename T, bool WRITE>
 cudaError_t launch_rows_t(const CacheParams& c, const CacheBatch& b, const CacheRows& r, cudaStream_t s) {
