@@ -106,6 +106,7 @@ struct FwdParams {
   uint32_t* drop_mask;   // tcgen05 attention(): the mask in memory (mask_word), or null
   int mask_drawn;        // launch_dropout_mask has drawn it; 0: the forward kernel draws it and leaves it there
   int window, sinks;     // window > 0: a row sees its last `window` keys and the first `sinks` (causal is 1 then)
+  int pair_heads;        // set by the tcgen05 launcher, windows: a CTA's query tiles are the same rows of two heads (1) or not (0)
   int early_tiles;       // tcgen05 score launches: the first tiles fetched into L2 before the wait on the previous kernel
 };
 

@@ -271,15 +271,17 @@ inline const LaunchFit& launch_fit(bool d128, RowChoiceKind kind, int rows) {
 // A lower bound of the launch's makespan, one CTA per SM at a time (the longest CTA, the mean load, and what the j SMs + 1
 // longest CTAs force onto one SM), lengthened where it takes several waves of unequal CTAs.  The row blocks of a head get
 // heavier towards its end (causal) or are alike, and every head has the same ones.
-inline double expected_us(const RowChoice& c, bool d128, RowChoiceKind kind, int rows) {
+// (`block`: the rows of a head that a CTA of `rows` rows has, fewer where it has several heads')
+inline double expected_us(const RowChoice& c, bool d128, RowChoiceKind kind, int rows, int block = 0) {
   const LaunchFit& f = launch_fit(d128, kind, rows);
-  const int ncb = c.blocks(rows);
+  if (block == 0) block = rows;
+  const int ncb = c.blocks(block);
   const long long n = ncb * c.heads;
   auto job = [&](int cb) -> double {
-    const int end = std::min(c.m_begin + (cb + 1) * rows, c.m_end);
+    const int end = std::min(c.m_begin + (cb + 1) * block, c.m_end);
     const int hi = c.causal ? std::max(0, std::min(c.N, c.p_seq + end)) : c.N;
     int tiles = (hi + kPlanTile - 1) / kPlanTile;
-    if (c.window > 0) tiles = key_tiles(c.m_begin + cb * rows, end, c.p_seq, c.N, c.window, c.sinks).count();
+    if (c.window > 0) tiles = key_tiles(c.m_begin + cb * block, end, c.p_seq, c.N, c.window, c.sinks).count();
     const bool ragged = cb == ncb - 1 && (c.m_end - c.m_begin) % kPlanTile != 0;
     return tiles == 0 ? f.empty : f.fix + (f.per + (ragged ? f.ragged : 0.0)) * tiles;
   };

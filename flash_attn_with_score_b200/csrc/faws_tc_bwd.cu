@@ -526,6 +526,20 @@ tc_bwd_kernel(const __grid_constant__ BwMaps maps, const BwTcParams p, int* __re
       tmem_ld32(t_s, reinterpret_cast<uint32_t(&)[32]>(sv[0]));
       tmem_ld32(t_s + 32, reinterpret_cast<uint32_t(&)[32]>(sv[32]));
       tmem_wait_ld();
+      if constexpr (kMasked && WIN) {
+        // Hidden entries become -inf here, and their weights zero below, 32 columns at a time and only where a row of the warp
+        // hides one.
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          auto below = [](int n) -> uint32_t { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u; };
+          const uint32_t word = below(x_hi + 1 - c * 32) & (~below(x_lo - c * 32) | (KM ? 0u : below(x_sink - c * 32)));
+          if (!__all_sync(0xffffffffu, word == ~0u)) {
+#pragma unroll
+            for (int x = 0; x < 32; ++x)
+              if (!(word >> x & 1u)) sv[c * 32 + x] = 0xff800000u;
+          }
+        }
+      }
       if (!KM) {  // the next tile's S' may be written
         tc_fence_before();
         mbar_arrive(&bars->s_free);
@@ -549,7 +563,7 @@ tc_bwd_kernel(const __grid_constant__ BwMaps maps, const BwTcParams p, int* __re
 #pragma unroll
           for (int y = 0; y < 4; ++y) {
             float pe = fast_exp2(t[y]);
-            if (kMasked && !(((x + y >= x_lo) || (WIN && !KM && x + y < x_sink)) && x + y <= x_hi)) pe = 0.f;
+            if (kMasked && !WIN && !(x + y >= x_lo && x + y <= x_hi)) pe = 0.f;
             sv[x + y] = __float_as_uint(pe);
             pr[y] = pe;
             // a product, not a select: a weight that is not finite stays visible where it is dropped

@@ -181,7 +181,12 @@ tc_fwd_kernel(const __grid_constant__ TcMaps maps, const FwdParams p, const __gr
   const int pack_m = FEW ? p.pack_m : 0;
   // WIN: attention_with_window().  A row sees its last p.window keys and the first p.sinks; the item's key tiles are a list (KeyTiles)
   // of those that hold sinks and those of its rows' windows, and kt0, nt and split ranges count along that list.
+  // pair: a 256-row CTA's two query tiles are the same 128 rows of two query heads of a group, so that they visit the same key
+  // tiles.  With rows one after the other each of them sits out a step of its own at one end of the window, and a step takes
+  // nearly as long for one tile as for two (fp16 B2 Hq16 Hk4 S2048 D64, window 512, 4 sinks: 34.5 us, paired 31.5).
   static_assert(!WIN || (HOOK == kHookNone && DROP == kNoDrop), "attention() without dropout");
+  const int pair = WIN && !SPLIT ? p.pair_heads : 0;
+  const int item_rows = pair ? BM : CTA_ROWS;
   const bool persist = !SPLIT && !kStoreHook && wl.n_items > 0;  // (the launcher keeps the other instances plain)
   bool is_fill;
   int cb_rel, h, b, ksplit, kt0, hk, bh, ho, cb_abs, nt, rr_start;
@@ -194,7 +199,7 @@ tc_fwd_kernel(const __grid_constant__ TcMaps maps, const FwdParams p, const __gr
     const int ncb = (p.lpt_order ? gz : gx) >> (p.fill_ctas ? 1 : 0);
     is_fill = p.fill_ctas && slot >= ncb;
     cb_rel = is_fill ? slot - ncb : ncb - 1 - slot;  // compute: heaviest (last) blocks first
-    h = p.lpt_order ? ix : iy;
+    h = (p.lpt_order ? ix : iy) << pair;
     // Split-KV launches (n_splits > 1) fold the key-range index into the batch axis of the grid.
     const int bz = p.lpt_order ? iy : iz;
     b = bz / p.n_splits;
@@ -203,8 +208,8 @@ tc_fwd_kernel(const __grid_constant__ TcMaps maps, const FwdParams p, const __gr
     hk = h / p.G;
     bh = b * p.Hq + h;
     ho = h * p.n_splits + ksplit;  // head index of the (partial) output the item writes
-    r_tile_of[0] = p.m_begin + cb_rel * CTA_ROWS;
-    r_tile_of[1] = r_tile_of[0] + (SPLIT ? 0 : BM);
+    r_tile_of[0] = p.m_begin + cb_rel * item_rows;
+    r_tile_of[1] = r_tile_of[0] + (SPLIT || pair ? 0 : BM);
     cb_abs = r_tile_of[0] / CTA_ROWS;  // start offset of the round-robin key-tile order
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
@@ -226,7 +231,7 @@ tc_fwd_kernel(const __grid_constant__ TcMaps maps, const FwdParams p, const __gr
     nt = max(nt_q[0], nt_q[1]) - kt0;  // key tiles the item visits
     if constexpr (WIN) {
       const int r0 = r_tile_of[0];
-      const int first = pack_m > 0 ? 0 : r0, end = pack_m > 0 ? pack_m : min(r0 + CTA_ROWS, p.m_end);
+      const int first = pack_m > 0 ? 0 : r0, end = pack_m > 0 ? pack_m : min(r0 + item_rows, p.m_end);
       kts = key_tiles(first, end, p.p_seq, p.N, p.window, p.sinks);
       sink_tiles = (p.sinks + BN - 1) / BN;
       nt = max(0, min(kts.count() - kt0, p.tiles_per_split));
@@ -393,7 +398,7 @@ tc_fwd_kernel(const __grid_constant__ TcMaps maps, const FwdParams p, const __gr
       for (int t = 0; t < L::kQTiles; ++t)
         for (int c = 0; c < D / 64; ++c)
           tma_load_4d(smem + L::q_off + t * L::kTile + c * L::kSub, &maps.q, &bars->q_full, c * 64,
-                      r_tile_of[t] - p.m_begin, h, b);
+                      r_tile_of[t] - p.m_begin, h + pair * t, b);
       for (int idx = 0; idx < n_early; ++idx) issue_kv_load(idx, idx);
     }
   }
@@ -432,7 +437,7 @@ tc_fwd_kernel(const __grid_constant__ TcMaps maps, const FwdParams p, const __gr
           for (int t = 0; t < L::kQTiles; ++t)
             for (int c = 0; c < D / 64; ++c)
               tma_load_4d(smem + L::q_off + t * L::kTile + c * L::kSub, &maps.q, &bars->q_full, c * 64,
-                          r_tile_of[t] - p.m_begin, h, b);
+                          r_tile_of[t] - p.m_begin, h + pair * t, b);
         }
         for (int idx = (k == 0 ? n_early : 0); idx < 2 * nt; ++idx) {
           const int g = ring_base + idx;
@@ -687,6 +692,7 @@ tc_fwd_kernel(const __grid_constant__ TcMaps maps, const FwdParams p, const __gr
     };
     auto tile_body = [&](auto masked_tag, int cnt, int n0) -> bool {
       constexpr bool kMasked = decltype(masked_tag)::value;
+      [[maybe_unused]] int live = 0xf;  // WIN: the chunks of 32 columns that some row of the warp sees
       // Masked tiles, one or two to a query tile, take their columns 32 at a time in rolled loops and read S again for the
       // exponentials: a quarter of the code, with which visible tiles share the instruction caches.  fp16 B16 H8 S785 D32 with
       // softmax column sums 108.6 -> 107.2 us, B4 H16 S1024 D64 with dropout (both passes) 192.5 -> 190.9, bf16 Hq28 Hk4 S4096
@@ -704,22 +710,7 @@ tc_fwd_kernel(const __grid_constant__ TcMaps maps, const FwdParams p, const __gr
         if (p.causal) lim = min(lim, FEW || WIN ? vis_end : i + p.p_seq + 1);
         nvis = max(0, min(128, lim - n0));
       }
-      // WIN: the window's keys of the row are columns [xlo, nvis), the sinks those before xsink.  Bit x of vis_word[c]: the row
-      // sees column 32 c + x; bit c of live: some row of the warp sees one of the 32.  Chunks that none sees are not
-      // exponentiated: of the 16 of a query tile a window's first and last key tile have ten, a tile of a few sinks four.
-      [[maybe_unused]] uint32_t vis_word[4] = {0u, 0u, 0u, 0u};
-      [[maybe_unused]] int live = 0xf;
-      if constexpr (kMasked && WIN) {
-        auto below = [](int n) -> uint32_t { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u; };
-        const int xlo = vis_end - p.window - n0, xsink = p.sinks - n0;
-        live = 0;
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          vis_word[c] = below(nvis - c * 32) & (~below(xlo - c * 32) | below(xsink - c * 32));
-          live |= __any_sync(0xffffffffu, vis_word[c] != 0u) ? 1 << c : 0;
-        }
-      }
-#define FAWS_VIS(x) (!kMasked || (WIN ? (vis_word[(x) >> 5] >> ((x) & 31) & 1u) != 0u : (x) < nvis))
+#define FAWS_VIS(x) (!kMasked || WIN || (x) < nvis)  // (windows: the hidden scores are -inf by then)
 
       // ---- row max (4 independent chains)
       float a0 = FAWS_NEG_INF, a1 = FAWS_NEG_INF, a2 = FAWS_NEG_INF, a3 = FAWS_NEG_INF;
@@ -756,10 +747,27 @@ tc_fwd_kernel(const __grid_constant__ TcMaps maps, const FwdParams p, const __gr
 #pragma unroll
         for (int c = 0; c < 4; ++c) tmem_ld32(t_s + c * 32, reinterpret_cast<uint32_t(&)[32]>(r[c * 32]));
         tmem_wait_ld();
+        if constexpr (kMasked && WIN) {
+          // Hidden scores become -inf, whose weights are zero: of the 16 chunks (a warp's rows, 32 columns) of a window's first or
+          // last tile six are hidden and four hidden in part, and the others cost what they cost elsewhere.  (Tests of every
+          // column where it is used: fp16 B2 Hq16 Hk4 S2048 D64 window 256 22.4 us, 20.7 so.)
+          auto below = [](int n) -> uint32_t { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u; };
+          const int lo = vis_end - p.window - n0, sink = p.sinks - n0;
+          live = 0;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const uint32_t word = below(nvis - c * 32) & (~below(lo - c * 32) | below(sink - c * 32));
+            if (__any_sync(0xffffffffu, word != 0u)) live |= 1 << c;
+            if (!__all_sync(0xffffffffu, word == ~0u)) {
+#pragma unroll
+              for (int x = 0; x < 32; ++x)
+                if (!(word >> x & 1u)) r[c * 32 + x] = 0xff800000u;
+            }
+          }
+        }
 #define FAWS_SV(x) (FAWS_VIS(x) ? __uint_as_float(r[x]) : FAWS_NEG_INF)
 #pragma unroll
         for (int x = 0; x < 128; x += 8) {  // three-input max: 64 instructions for 128 values
-          if (kMasked && WIN && !(live >> (x >> 5) & 1)) continue;
           a0 = fmax3(a0, FAWS_SV(x), FAWS_SV(x + 1));
           a1 = fmax3(a1, FAWS_SV(x + 2), FAWS_SV(x + 3));
           a2 = fmax3(a2, FAWS_SV(x + 4), FAWS_SV(x + 5));
@@ -1297,13 +1305,13 @@ tc_fwd_kernel(const __grid_constant__ TcMaps maps, const FwdParams p, const __gr
           __syncwarp();
           if (lane == 0) {
             for (int sub = 0; sub < D / 64; ++sub)
-              tma_store_4d(&maps.o, ost + sub * 4096, sub * 64, r_tile + lg * 32 - p.m_begin, ho, b);
+              tma_store_4d(&maps.o, ost + sub * 4096, sub * 64, r_tile + lg * 32 - p.m_begin, ho + pair * qt, b);
             tma_store_commit();
           }
         }
       } else if (row_ok && !(FEW && p.n_splits > 1)) {  // (the combine leaves out ranges with L = -inf)
         // no key is visible to this query tile: its rows are zero
-        T* orow = reinterpret_cast<T*>(p.o) + b * p.o_sb + ho * p.o_sh + (int64_t)i * p.o_ss;
+        T* orow = reinterpret_cast<T*>(p.o) + b * p.o_sb + (ho + pair * qt) * p.o_sh + (int64_t)i * p.o_ss;
         const uint4 z = make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
         for (int g = 0; g < D / 8; ++g)
@@ -1311,7 +1319,7 @@ tc_fwd_kernel(const __grid_constant__ TcMaps maps, const FwdParams p, const __gr
       }
       if (row_ok) {
         if (p.L != nullptr)
-          p.L[((int64_t)bh * p.n_splits + ksplit) * p.M + i] = l_all > 0.f ? (m_all + log2f(l_all)) * kLn2 : FAWS_NEG_INF;
+          p.L[((int64_t)(bh + pair * qt) * p.n_splits + ksplit) * p.M + i] = l_all > 0.f ? (m_all + log2f(l_all)) * kLn2 : FAWS_NEG_INF;
         if constexpr (HOOK == kHookRowSum) p.row_sum[(int64_t)bh * p.M + i] = rs_all;
       }
     }
@@ -1382,7 +1390,8 @@ cudaError_t launch_fwd_s(const TcMaps& maps, const FwdParams& p, cudaStream_t s)
   static PerDeviceOnce attr_once;
   if (cudaError_t e = set_max_smem_once(attr_once, tc_fwd_kernel<T, D, HOOK, SPLIT, DROP, FEW, WIN>, L::alloc); e != cudaSuccess)
     return e;
-  const int ncb = (p.m_end - p.m_begin + L::kRows - 1) / L::kRows;
+  const int pair = WIN && !SPLIT ? p.pair_heads : 0, rows = pair ? BM : L::kRows;
+  const int ncb = (p.m_end - p.m_begin + rows - 1) / rows, heads = p.Hq >> pair;
   FwdParams pp = p;
   // K and V of all heads together stay resident in the 126 MB L2 -> order CTAs for load balance
   const long long kv_bytes = 2LL * p.B * p.Hk * p.N * p.D * 2;
@@ -1404,13 +1413,13 @@ cudaError_t launch_fwd_s(const TcMaps& maps, const FwdParams& p, cudaStream_t s)
   if (pp.schedule == kRoundRobin && pp.causal) pp.schedule = kReverse;
   if (pp.n_splits < 1) pp.n_splits = 1;
   if (pp.n_splits == 1) pp.tiles_per_split = (p.N + BN - 1) / BN;  // (no shorter than a list of them)
-  dim3 grid = pp.lpt_order ? dim3(p.Hq, p.B * pp.n_splits, nslots) : dim3(nslots, p.Hq, p.B * pp.n_splits);
+  dim3 grid = pp.lpt_order ? dim3(heads, p.B * pp.n_splits, nslots) : dim3(nslots, heads, p.B * pp.n_splits);
   // Tensor-bound launches with more items than SMs: one persistent CTA per SM walks a work list.
   WorkList wl_persist;
   const WorkList* wl = &plain_work_list();
   if constexpr (!SPLIT && (HOOK == kHookNone || HOOK == kHookRowSum || HOOK == kHookColPart)) {
     const WorkShape shape{(int)grid.x, (int)grid.y, (int)grid.z, pp.lpt_order, pp.causal, pp.p_seq, pp.m_begin, pp.m_end,
-                          pp.N, L::kRows, sm_count(), pp.pack_m, WIN ? pp.window : 0, pp.sinks};
+                          pp.N, rows, sm_count(), pp.pack_m, WIN ? pp.window : 0, pp.sinks};
     if (pp.n_splits == 1 && !pp.fill_ctas && persistent_allowed() && make_work_list(shape, &wl_persist)) {
       wl = &wl_persist;
       grid = dim3(sm_count(), 1, 1);

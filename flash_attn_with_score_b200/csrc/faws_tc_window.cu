@@ -10,9 +10,16 @@ namespace {
 template <typename T, int D>
 cudaError_t launch_t(const TcMaps& maps, const FwdParams& p, cudaStream_t s) {
   if (p.pack_m > 0 || p.n_splits > 1) return launch_fwd_s<T, D, kHookNone, true, kNoDrop, true, true>(maps, p, s);
-  const RowChoice c{(long long)p.B * p.Hq, p.m_begin, p.m_end, p.N, p.p_seq, p.causal, sm_count(), p.window, p.sinks};
-  const bool large = c.blocks(256) * c.heads >= 2LL * c.sms || prefer_256_rows(c, D == 128, kPlainOut);
-  return large ? launch_fwd_s<T, D, kHookNone, false, kNoDrop, false, true>(maps, p, s)
+  // 256-row CTAs, of two heads' rows where the group has an even number of them, against 128-row ones by the times that plain
+  // launches of as many key tiles are expected to take.
+  FwdParams pp = p;
+  pp.pair_heads = p.G % 2 == 0 ? 1 : 0;
+  RowChoice c{(long long)p.B * p.Hq, p.m_begin, p.m_end, p.N, p.p_seq, p.causal, sm_count(), p.window, p.sinks};
+  const double small = expected_us(c, D == 128, kPlainOut, 128);
+  if (pp.pair_heads) c.heads /= 2;
+  const bool large = c.blocks(pp.pair_heads ? 128 : 256) * c.heads >= 2LL * c.sms ||
+                     small > 1.03 * expected_us(c, D == 128, kPlainOut, 256, pp.pair_heads ? 128 : 0);
+  return large ? launch_fwd_s<T, D, kHookNone, false, kNoDrop, false, true>(maps, pp, s)
                : launch_fwd_s<T, D, kHookNone, true, kNoDrop, false, true>(maps, p, s);
 }
 
