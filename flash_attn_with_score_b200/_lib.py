@@ -33,6 +33,7 @@ EXPORTS = [
     "faws_attention_with_softmax_col_sum", "faws_attention_cross_token_qk_sum",
     "faws_attention_cross_token_softmax_sum", "faws_attention_cross_token_softmax_sum_buffered",
     "faws_window_split_plan", "faws_attention_with_window", "faws_attention_with_window_backward",
+    "faws_window_backward_bytes",
     "faws_kv_cache_write", "faws_kv_cache_read", "faws_attention_with_kv_cache", "faws_kv_cache_workspace_bytes",
     "faws_total_attention", "faws_attention_backward", "faws_workspace_bytes", "faws_reduce_ranks", "faws_device_status",
     "faws_selftest_wait_give_up", "faws_last_backend",
@@ -112,6 +113,7 @@ def load():
         "faws_window_split_plan": (i32, [PP, i32, i32]),
         "faws_attention_with_window": (i32, [PP, i32, i32, i32, vp, sz, vp]),
         "faws_attention_with_window_backward": (i32, [PP, C.POINTER(Grads), i32, i32, vp, sz, vp]),
+        "faws_window_backward_bytes": (sz, [PP, i32, i32]),
         "faws_kv_cache_write": (i32, cache + [C.POINTER(Tensor), C.POINTER(Tensor), i32, vp]),
         "faws_kv_cache_read": (i32, cache + [C.POINTER(Tensor), C.POINTER(Tensor), i32, vp]),
         "faws_attention_with_kv_cache": (i32, [PP] + cache + [i32, i32, vp, sz, vp]),

@@ -268,7 +268,8 @@ class _WindowFunction(torch.autograd.Function):
         c = _Call(q, k, v, True, ctx.sm_scale, 0.0, out=o, L=L, backend=ctx.backend)
         dq, dk, dv = torch.empty_like(c.q), torch.empty_like(c.k), torch.empty_like(c.v)
         g = _lib.Grads(_tensor(do), _tensor(dq), _tensor(dk), _tensor(dv))
-        ws, n = c.workspace(_lib.OP_ATTENTION_BACKWARD)
+        n = c.lib.faws_window_backward_bytes(C.byref(c.p), ctx.window, ctx.sinks)
+        ws = torch.empty(n, device=c.dev, dtype=torch.uint8)
         c.run("faws_attention_with_window_backward", C.byref(g), ctx.window, ctx.sinks, C.c_void_p(ws.data_ptr()), n)
         return dq, dk, dv, None, None, None, None, None
 

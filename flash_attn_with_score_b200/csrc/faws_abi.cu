@@ -719,9 +719,10 @@ static int backward(const faws_problem* p, const faws_grads* g, const void* mask
   if (p->m_begin != 0 || p->m_end != p->M) return FAWS_EINVAL;
   // Scratch sized for the same shape with 16-bit partial gradients (before dropout was turned on) is enough for the
   // CUDA-core kernels, which then run unless the family is forced.
-  const size_t least = tc_bwd_workspace_bytes(p->B, p->Hq, p->Hk, p->M, p->N, p->D, false);
+  const size_t least = window > 0 ? tc_bwd_window_bytes(p->B, p->Hq, p->Hk, p->M, p->N, p->D, window, sinks)
+                                  : tc_bwd_workspace_bytes(p->B, p->Hq, p->Hk, p->M, p->N, p->D, false);
   // Without room for the dropout mask the kernels draw it as they go.
-  const size_t need = tc_bwd_workspace_bytes(p->B, p->Hq, p->Hk, p->M, p->N, p->D, p->dropout_p > 0.f || p->D < 64);
+  const size_t need = window > 0 ? least : tc_bwd_workspace_bytes(p->B, p->Hq, p->Hk, p->M, p->N, p->D, p->dropout_p > 0.f || p->D < 64);
   if (workspace == nullptr || workspace_bytes < least || misaligned_ws(workspace)) return FAWS_EWORKSPACE;
   BwdParams b{};
   b.q = p->q.ptr; b.k = p->k.ptr; b.v = p->v.ptr; b.o = p->out.ptr;
@@ -816,6 +817,11 @@ int faws_attention_with_window(const faws_problem* p, int32_t window, int32_t si
     return FAWS_ECUDA;
   t_last_backend = FAWS_BACKEND_TCGEN05;
   return FAWS_OK;
+}
+
+size_t faws_window_backward_bytes(const faws_problem* p, int32_t window, int32_t sinks) {
+  if (validate_window(p, window, sinks) != FAWS_OK) return 0;
+  return tc_bwd_window_bytes(p->B, p->Hq, p->Hk, p->M, p->N, p->D, clamp_span(window), clamp_span(sinks));
 }
 
 int faws_attention_with_window_backward(const faws_problem* p, const faws_grads* g, int32_t window, int32_t sinks,

@@ -280,6 +280,7 @@ bool tc_bwd_supported(const BwdParams& p, int dtype);
 cudaError_t launch_tc_bwd(const BwdParams& p, int dtype, cudaStream_t s);  // p.delta = the workspace base
 // fine: with dropout or a head dim below 64 (fp32 partials, statistics of the pre-pass)
 size_t tc_bwd_workspace_bytes(int B, int Hq, int Hk, int M, int N, int D, bool fine);
+size_t tc_bwd_window_bytes(int B, int Hq, int Hk, int M, int N, int D, int window, int sinks);
 size_t tc_bwd_mask_bytes(int B, int Hq, int M, int N);  // of the dropout mask of the heads that take a turn; 0 where none is kept
 
 int tc_read_status(int reset);  // synchronising read of the device status word

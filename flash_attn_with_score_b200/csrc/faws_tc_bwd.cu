@@ -118,6 +118,11 @@ struct BwTcParams {
   const uint32_t* mask;  // dropout: the mask as the pre-pass has drawn it (see draw_mask), or null
   int bh0;               // dropout: the launch's first (batch, head)
   int window, sinks;     // WIN: a query sees its last `window` keys and the first `sinks`
+  // WIN, key-major, where loop > 0 (WindowPlan): a CTA walks the loop (all G) query heads of its kv head, so that dK and dV of a
+  // key tile need no other CTA's.  Tiles with sinks, which every query sees, are cut into parts instead, a query head and one of
+  // `ranges` of the query tiles each, whose fp32 results (B,Hk,parts of a tile,sink_rows,D) another kernel adds up.
+  int loop, sink_tiles, ranges, sink_rows;
+  float *sink_dv, *sink_dk;
 };
 
 // The dropout mask (mask_word) in scratch, where the forward pass kept none.  Both kernels need it, and a kernel with nothing else to
@@ -208,12 +213,28 @@ tc_bwd_kernel(const __grid_constant__ BwMaps maps, const BwTcParams p, int* __re
   // Heaviest work first in launch order: key-major, the first key tiles see the most queries when
   // causal; query-major, the last query tiles see the most keys.
   const int own_tiles = (int)gridDim.z;
-  const int own_tile = KM ? (int)blockIdx.z : (p.causal ? own_tiles - 1 - (int)blockIdx.z : (int)blockIdx.z);
+  int own_tile = KM ? (int)blockIdx.z : (p.causal ? own_tiles - 1 - (int)blockIdx.z : (int)blockIdx.z);
   int h = blockIdx.x, b = blockIdx.y;
   if constexpr (MODE == kDrop) {  // the heads of a launch are consecutive, of several batches maybe
     const int bh = p.bh0 + b * (int)gridDim.x + h;
     b = bh / p.Hq;
     h = bh - b * p.Hq;
+  }
+  // heads h .. h + loop - 1 are walked; a part of a tile with sinks: its number, and its share of the query tiles
+  [[maybe_unused]] int loop = 1, part_no = -1;
+  if constexpr (WIN && KM) {
+    if (p.loop > 0) {  // grid: (kv heads, batches, the parts of tiles with sinks, then the other tiles)
+      const int per_tile = p.loop * p.ranges, parts = p.sink_tiles * per_tile, z = (int)blockIdx.z;
+      h *= p.G;
+      if (z < parts) {
+        own_tile = z / per_tile;
+        part_no = z - own_tile * per_tile;
+        h += part_no / p.ranges;
+      } else {
+        own_tile = p.sink_tiles + z - parts;
+        loop = p.loop;
+      }
+    }
   }
   const int hk = h / p.G;
   const int own0 = own_tile * BT;  // first owned row: key n0 (key-major) or query i0 (query-major)
@@ -226,6 +247,11 @@ tc_bwd_kernel(const __grid_constant__ BwMaps maps, const BwTcParams p, int* __re
     // the last query that sees a key of the tile is the one at the end of its last key's window; sinks are seen by all
     if (WIN && own0 >= p.sinks) m_end = max(0, min(p.M, own0 + BT - 1 - p.p_seq + p.window));
     nu = max(0, (m_end + BT - 1) / BT - u0);
+    if (WIN && part_no >= 0) {
+      const int per = (nu + p.ranges - 1) / p.ranges, skip = min(nu, part_no % p.ranges * per);
+      u0 += skip;
+      nu = min(per, nu - skip);
+    }
   } else {
     int hi = p.N;
     if (p.causal) hi = max(0, min(p.N, p.p_seq + min(own0 + BT, p.M)));
@@ -240,6 +266,8 @@ tc_bwd_kernel(const __grid_constant__ BwMaps maps, const BwTcParams p, int* __re
     if constexpr (WIN && !KM) return kts.tile(u) * BT;
     return (u0 + u) * BT;
   };
+
+  const int total = WIN && KM ? loop * nu : nu;  // streamed tiles of all heads
 
   // Launch chain: pre-pass, query-major, key-major, group sum, each allowed to begin while the one before it drains.
   // Only the key-major kernel's partials and the pre-pass's arrays pass between them: the query-major kernel waits
@@ -299,23 +327,34 @@ tc_bwd_kernel(const __grid_constant__ BwMaps maps, const BwTcParams p, int* __re
         for (int c = 0; c < D / 64; ++c) tma_load_4d(smem + at + c * L::kSub, m, bar, c * 64, row0, head, b);
       };
       load_tile(L::x_off, &maps.x, &bars->x_full, own0, x_head);
-      for (int u = 0; u < nu; ++u) {
-        const int row0 = first_row(u), sa = u % NA, sb = u % NB;
+      [[maybe_unused]] int head = a_head, ut = 0;  // of streamed tile u
+      for (int u = 0; u < total; ++u) {
+        const int row0 = first_row(WIN && KM ? ut : u), sa = u % NA, sb = u % NB;
         if (u >= NA && !mbar_wait(&bars->a_empty[sa], (u / NA - 1) & 1, abort_flag)) break;
-        load_tile(L::a_off + sa * L::kTile, &maps.a, &bars->a_full[sa], row0, a_head);
+        load_tile(L::a_off + sa * L::kTile, &maps.a, &bars->a_full[sa], row0, WIN && KM ? head : a_head);
         if (u == 0) load_tile(L::y_off, &maps.y, &bars->y_full, own0, x_head);
         if (u >= NB && !mbar_wait(&bars->b_empty[sb], (u / NB - 1) & 1, abort_flag)) break;
-        load_tile(L::b_off + sb * L::kTile, &maps.b, &bars->b_full[sb], row0, a_head);
+        load_tile(L::b_off + sb * L::kTile, &maps.b, &bars->b_full[sb], row0, WIN && KM ? head : a_head);
+        if (WIN && KM && ++ut == nu) {
+          ut = 0;
+          ++head;
+        }
       }
     } else if (KM && warp == 2 && lane == 0) {
       // ---------------------------------------------------------- L and delta of the streamed query tiles
-      for (int u = 0; u < nu; ++u) {
+      [[maybe_unused]] int64_t row = vec_row;
+      [[maybe_unused]] int ut = 0;
+      for (int u = 0; u < total; ++u) {
         const int s = u & 1;
         if (u >= 2 && !mbar_wait(&bars->vec_empty[s], (u / 2 - 1) & 1, abort_flag)) break;
-        const int64_t at = vec_row + (u0 + u) * BT;
+        const int64_t at = WIN ? row + (u0 + ut) * BT : vec_row + (u0 + u) * BT;
         mbar_arrive_expect_tx(&bars->vec_full[s], 1024);
         bulk_load_1d(smem + L::vec_off + s * 1024, p.negl2 + at, 512, &bars->vec_full[s]);
         bulk_load_1d(smem + L::vec_off + s * 1024 + 512, p.neg_delta + at, 512, &bars->vec_full[s]);
+        if (WIN && ++ut == nu) {
+          ut = 0;
+          row += p.Mpad;
+        }
       }
     } else if (warp == 1 && nu > 0 && elect_one()) {
       // ---------------------------------------------------------- MMA issuer: one thread
@@ -390,8 +429,8 @@ tc_bwd_kernel(const __grid_constant__ BwMaps maps, const BwTcParams p, int* __re
       wait(&bars->y_full, 0);
       issue_dp(0);
       if (!KM && ok) mma_commit(&bars->b_empty[0]);
-      for (int u = 0; ok && u < nu; ++u) {
-        const bool more = u + 1 < nu;
+      for (int u = 0; ok && u < total; ++u) {
+        const bool more = u + 1 < total;
         if constexpr (KM) {
           if (NSB == 2 && more) issue_s(u + 1);
 #pragma unroll
@@ -469,9 +508,8 @@ tc_bwd_kernel(const __grid_constant__ BwMaps maps, const BwTcParams p, int* __re
     }
 
     // One streamed tile, kMasked where an entry of this warpgroup's 128 x 64 block may be hidden.
-    auto tile_body = [&](auto masked_tag, int u) -> bool {
+    auto tile_body = [&](auto masked_tag, int u, int str0) -> bool {  // str0: first streamed row of this half
       constexpr bool kMasked = decltype(masked_tag)::value;
-      const int str0 = first_row(u) + e * HALF;  // first streamed row of this half
       // causal: (query i, key j) is visible iff j <= i + p_seq.  Column x of the half is streamed row
       // str0 + x.  Key-major (own = j, streamed = i): visible iff x >= own - p_seq - str0.
       // Query-major (own = i, streamed = j): visible iff x <= own + p_seq - str0.
@@ -649,8 +687,10 @@ tc_bwd_kernel(const __grid_constant__ BwMaps maps, const BwTcParams p, int* __re
       return true;
     };
     bool alive = true;
-    for (int u = 0; alive && u < nu; ++u) {
-      const int str0 = first_row(u) + e * HALF;
+    [[maybe_unused]] int ut = 0;
+    for (int u = 0; alive && u < total; ++u) {
+      const int str0 = first_row(WIN && KM ? ut : u) + e * HALF;
+      if (WIN && KM && ++ut == nu) ut = 0;
       bool masked;
       if (KM) masked = (p.causal && own0 + BT - 1 - p.p_seq > str0) || (MODE == kDrop && str0 + HALF > p.M);
       else masked = str0 + HALF > (p.causal ? min(p.N, own0 + p.p_seq + 1) : p.N);
@@ -658,7 +698,7 @@ tc_bwd_kernel(const __grid_constant__ BwMaps maps, const BwTcParams p, int* __re
         if (KM) masked = masked || (own0 + BT > p.sinks && str0 + HALF - 1 > max(own0, p.sinks) - p.p_seq + p.window - 1);
         else masked = masked || (str0 + HALF > p.sinks && str0 < own0 + BT + p.p_seq - p.window);
       }
-      alive = masked ? tile_body(std::true_type{}, u) : tile_body(std::false_type{}, u);
+      alive = masked ? tile_body(std::true_type{}, u, str0) : tile_body(std::false_type{}, u, str0);
     }
 
     // ---- epilogue: accumulators -> 16-bit -> swizzled smem -> TMA store (clips at the tensor's edge)
@@ -686,6 +726,19 @@ tc_bwd_kernel(const __grid_constant__ BwMaps maps, const BwTcParams p, int* __re
 #pragma unroll
             for (int x = 0; x < 32; ++x) ro[x] = 0u;  // no streamed tile at all: the gradient rows are zero
           }
+          if constexpr (WIN && KM) {
+            if (part_no >= 0) {
+              const int64_t row = (((int64_t)b * (p.Hq / p.G) + hk) * (p.loop * p.ranges) + part_no) * p.sink_rows + own;
+              float* dst = (e == 0 ? p.sink_dv : p.sink_dk) + row * D + sub * 64 + c * 32;
+#pragma unroll
+              for (int g = 0; g < 8; ++g)
+                if (own < p.sink_rows)
+                  *reinterpret_cast<float4*>(dst + g * 4) =
+                      make_float4(__uint_as_float(ro[g * 4]) * oscale, __uint_as_float(ro[g * 4 + 1]) * oscale,
+                                  __uint_as_float(ro[g * 4 + 2]) * oscale, __uint_as_float(ro[g * 4 + 3]) * oscale);
+              continue;
+            }
+          }
           if constexpr (MODE != kPlain) {
             if (part != nullptr) {  // a row piece of up to 128 bytes per thread
               float* dst = part + (((int64_t)b * p.Hq + h) * p.N + own) * p.D + sub * 64 + c * 32;
@@ -712,10 +765,11 @@ tc_bwd_kernel(const __grid_constant__ BwMaps maps, const BwTcParams p, int* __re
       }
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0 && part == nullptr) {
+      if (lane == 0 && part == nullptr && part_no < 0) {
         const CUtensorMap* om = (KM && e == 1) ? &maps.o1 : &maps.o0;
+        const int head = WIN && KM && p.loop > 0 ? hk : h;
         for (int sub = sub_first; sub < D / 64; sub += sub_step)
-          tma_store_4d(om, ost + sub * 4096, sub * 64, own0 + lg * 32, h, b);
+          tma_store_4d(om, ost + sub * 4096, sub * 64, own0 + lg * 32, head, b);
         tma_store_commit();
         tma_store_wait<0>();
       }
@@ -984,6 +1038,39 @@ BwWs bwd_ws(int B, int Hq, int Hk, int M, int N, int D, bool fine) {
   return w;
 }
 
+// How dK and dV of a windowed problem are made (see BwTcParams::loop); loop 0: a CTA per query head, as without windows.
+// Walking a group's heads in one CTA spares its heads' partial gradients, their rounding to 16 bits and the launch that adds them, for
+// G times fewer and longer CTAs: taken where whole waves of those are expected to end no later.  bf16 Hq28 Hk4 S8192 D128, window
+// 1024, 4 sinks, dK and dV: 282 us a head at a time, 236 so; fp16 B2 H12 S1531 D64, window 300, 7 sinks, is better off without the
+// parts (57 us with the other kernels, 63 with).
+struct WindowPlan {
+  int loop, sink_tiles, ranges, parts, rows;  // parts: of a tile with sinks; rows: keys of these tiles
+};
+WindowPlan plan_window(int B, int Hq, int Hk, int M, int N, int D, int window, int sinks, int sms) {
+  const int G = Hq / Hk, nkt = (N + BT - 1) / BT, nqt = (M + BT - 1) / BT;
+  const int sink_tiles = (std::min(sinks, N) + BT - 1) / BT;
+  if (D < 64 || sink_tiles > 4) return {};
+  const int steps = std::min(nqt, std::min(window, N) / BT + 2);  // query tiles that see a key tile without sinks
+  WindowPlan w{G, sink_tiles, 1, 0, std::min(N, sink_tiles * BT)};
+  // parts of tiles with sinks no longer than the other CTAs, or than a few steps
+  if (sink_tiles > 0) w.ranges = std::max(1, std::min(8, nqt / std::max(4, G * steps)));
+  w.parts = G * w.ranges;
+  // Expected times, in streamed tiles, of a CTA for each query head and key tile (chains of all query tiles where there are sinks) and so
+  // (the CTAs of a wave being of a length), with the launch that adds up partials where there is one.
+  const long long others = (long long)(nkt - sink_tiles) * Hk * B, ctas = others + (long long)sink_tiles * w.parts * Hk * B;
+  const double step_us = D == 128 ? 1.8 : 1.3;
+  const double mean = ((double)others * G * steps + (double)sink_tiles * nqt * Hq * B) / sms;
+  const double sums = G > 1 ? (5.0 + 4.0 * B * Hq * (double)N * D * 2 / 6.0e6) / step_us : 0.0;  // two partials written and read
+  const double apart = std::max(mean, (double)(sink_tiles > 0 ? nqt : steps)) + sums;
+  const double looped = (G > 1 ? (double)((ctas + sms - 1) / sms) * G * steps : std::max(mean, (double)nqt / w.ranges)) +
+                        (sink_tiles > 0 ? 5.0 / step_us : 0.0);
+  if (looped >= apart) return {};
+  return w;
+}
+size_t window_ws_bytes(const WindowPlan& w, int B, int Hk, int D) {  // of either gradient's partials
+  return ((size_t)B * Hk * w.parts * w.rows * D * 4 + 255) & ~size_t(255);
+}
+
 template <typename T, int D, int MODE, bool WIN = false>
 cudaError_t launch_bwd_td(const BwdParams& p, cudaStream_t s) {
   using Lk = BwSmem<D, true>;
@@ -1025,12 +1112,19 @@ cudaError_t launch_bwd_td(const BwdParams& p, cudaStream_t s) {
   tp.mask = p.mask != nullptr ? p.mask : mask;
   tp.g_stat = st.g; tp.v_stat = st.v; tp.g_blocks = st.g_blocks; tp.v_blocks = st.v_blocks;
   int* status_word = tc_status_word();
-  const bool per_head = p.G > 1;
+  WindowPlan win{};
+  if constexpr (WIN) win = plan_window(p.B, p.Hq, p.Hk, p.M, p.N, p.D, p.window, p.sinks, sm_count());
+  const bool per_head = p.G > 1 && win.loop == 0;
   const bool map_parts = per_head && MODE == kPlain;  // 16-bit partials go through the store maps
   BwTcParams tk = tp;  // the key-major launches': with the fp32 partials
   if (per_head && !map_parts) {
     tk.part0 = reinterpret_cast<float*>(dv_part);
     tk.part1 = reinterpret_cast<float*>(dk_part);
+  }
+  if (WIN && win.loop > 0) {
+    tk.loop = win.loop; tk.sink_tiles = win.sink_tiles; tk.ranges = win.ranges; tk.sink_rows = win.rows;
+    tk.sink_dv = reinterpret_cast<float*>(base + ws.dk);
+    tk.sink_dk = reinterpret_cast<float*>(base + ws.dk + window_ws_bytes(win, p.B, p.Hk, p.D));
   }
   BwMaps qm, km;
   {  // query-major: dQ
@@ -1047,7 +1141,7 @@ cudaError_t launch_bwd_td(const BwdParams& p, cudaStream_t s) {
     BwMaps& m = km;
     void* dv_dst = map_parts ? static_cast<void*>(dv_part) : p.dv;
     void* dk_dst = map_parts ? static_cast<void*>(dk_part) : p.dk;
-    const int o_heads = per_head && !map_parts ? p.Hk : p.Hq;  // (those maps are not used with fp32 partials)
+    const int o_heads = (per_head && !map_parts) || win.loop > 0 ? p.Hk : p.Hq;  // (not used with fp32 partials)
     const int64_t ph_ss = p.D, ph_sh = (int64_t)p.N * p.D, ph_sb = (int64_t)p.Hq * p.N * p.D;
     if (!make_map_bhsd(&m.x, p.k, p.D, p.N, p.Hk, p.B, p.k_ss, p.k_sh, p.k_sb, 128) ||
         !make_map_bhsd(&m.y, p.v, p.D, p.N, p.Hk, p.B, p.v_ss, p.v_sh, p.v_sb, 128) ||
@@ -1067,8 +1161,16 @@ cudaError_t launch_bwd_td(const BwdParams& p, cudaStream_t s) {
     if ((e = launch_overlapped(tc_bwd_kernel<T, D, false, MODE, WIN>, dim3(gx, gy, (p.M + BT - 1) / BT), NTHREADS, Lq::total, s,
                                qm, tp, status_word)) != cudaSuccess)
       return e;
-    if ((e = launch_overlapped(tc_bwd_kernel<T, D, true, MODE, WIN>, dim3(gx, gy, (p.N + BT - 1) / BT), NTHREADS, Lk::total, s,
-                               km, tk, status_word)) != cudaSuccess)
+    const unsigned key_tiles = (p.N + BT - 1) / BT;
+    const dim3 kgrid = win.loop > 0 ? dim3(p.Hk, p.B, key_tiles - win.sink_tiles + win.sink_tiles * win.parts) : dim3(gx, gy, key_tiles);
+    if ((e = launch_overlapped(tc_bwd_kernel<T, D, true, MODE, WIN>, kgrid, NTHREADS, Lk::total, s, km, tk, status_word)) != cudaSuccess)
+      return e;
+  }
+  if (WIN && win.loop > 0 && win.sink_tiles > 0) {
+    const int64_t n = (int64_t)p.B * p.Hk * win.rows * (p.D / 8);
+    const GroupSumOut dk{p.dk, p.dk_sb, p.dk_sh, p.dk_ss}, dv{p.dv, p.dv_sb, p.dv_sh, p.dv_ss};
+    if ((e = launch_overlapped(bwd_group_sum_kernel<T, float>, dim3((unsigned)((n + 255) / 256), 2, 1), 256, 0, s,
+                               (const float*)tk.sink_dk, (const float*)tk.sink_dv, dk, dv, p.B, p.Hk, win.parts, win.rows, p.D)) != cudaSuccess)
       return e;
   }
   if (per_head) {
@@ -1098,6 +1200,12 @@ cudaError_t launch_bwd_t(const BwdParams& p, cudaStream_t s) {
 
 size_t tc_bwd_workspace_bytes(int B, int Hq, int Hk, int M, int N, int D, bool fine) {
   return bwd_ws(B, Hq, Hk, M, N, D, fine).total;
+}
+
+size_t tc_bwd_window_bytes(int B, int Hq, int Hk, int M, int N, int D, int window, int sinks) {
+  const WindowPlan w = plan_window(B, Hq, Hk, M, N, D, window, sinks, sm_count());
+  const BwWs ws = bwd_ws(B, Hq, Hk, M, N, D, D < 64);
+  return w.loop == 0 ? ws.total : ws.dk + 2 * window_ws_bytes(w, B, Hk, D);
 }
 
 size_t tc_bwd_mask_bytes(int B, int Hq, int M, int N) {

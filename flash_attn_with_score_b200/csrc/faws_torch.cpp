@@ -133,10 +133,10 @@ struct WindowFunction : public torch::autograd::Function<WindowFunction> {
     const at::Tensor Lc = L.contiguous();
     p.log_normalizer = Lc.data_ptr<float>();
     const faws_grads g{view(dout), view(dq), view(dk), view(dv)};
-    const size_t n = faws_workspace_bytes(FAWS_OP_ATTENTION_BACKWARD, &p, 0);
+    const int32_t window = (int32_t)ctx->saved_data["window"].toInt(), sinks = (int32_t)ctx->saved_data["sinks"].toInt();
+    const size_t n = faws_window_backward_bytes(&p, window, sinks);
     const at::Tensor ws = bytes_like(q, n);
-    check(faws_attention_with_window_backward(&p, &g, (int32_t)ctx->saved_data["window"].toInt(), (int32_t)ctx->saved_data["sinks"].toInt(),
-                                              ws.data_ptr(), n, current_stream(q)),
+    check(faws_attention_with_window_backward(&p, &g, window, sinks, ws.data_ptr(), n, current_stream(q)),
           "faws_attention_with_window_backward");
     return {dq, dk, dv, none, none, none};
   }

@@ -308,13 +308,15 @@ size_t faws_workspace_bytes(int32_t op, const faws_problem* p, int32_t split);
  * visits are cut into so many ranges.  faws_window_split_plan says how many the library would choose.
  * Workspace for n_splits > 1: faws_workspace_bytes(FAWS_OP_ATTENTION_SPLIT_KV, p, n_splits).
  *
- * Backward pass: as faws_attention_backward, with its workspace.  Keys that no query sees get zero gradients.
+ * Backward pass: as faws_attention_backward.  Keys that no query sees get zero gradients.  Workspace:
+ * faws_window_backward_bytes.
  */
 int32_t faws_window_split_plan(const faws_problem* p, int32_t window, int32_t sinks);
 int faws_attention_with_window(const faws_problem* p, int32_t window, int32_t sinks, int32_t n_splits, void* workspace,
                                size_t workspace_bytes, void* stream);
 int faws_attention_with_window_backward(const faws_problem* p, const faws_grads* g, int32_t window, int32_t sinks,
                                         void* workspace, size_t workspace_bytes, void* stream);
+size_t faws_window_backward_bytes(const faws_problem* p, int32_t window, int32_t sinks);
 
 /*
  * A paged cache of keys and values in 4 bits, and the operators on it.  No counterpart in the reference.

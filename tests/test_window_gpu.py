@@ -157,6 +157,21 @@ def test_many_row_blocks(shape):
     _check(shape, F16, backward=shape[1] < 100)
 
 
+@pytest.mark.parametrize("shape", [
+    (8, 4, 2, 1100, 1100, 64, 64, 4),      # a group's heads in one CTA, the tile with sinks in parts of heads and query ranges
+    (4, 14, 2, 1700, 1700, 64, 60, 200),   # two tiles with sinks
+    (1, 3, 3, 2500, 2500, 64, 90, 300),    # three, each in five ranges
+    (2, 16, 4, 900, 900, 128, 100, 0),     # none
+    (2, 6, 2, 300, 1200, 128, 50, 140),    # queries that begin behind the tiles with sinks
+    (2, 6, 2, 700, 300, 64, 50, 140),      # and before the first key
+    (1, 8, 2, 1100, 1100, 128, 64, 600),   # too many sinks for parts
+    (3, 32, 8, 300, 300, 64, 256, 4)],
+    ids=lambda s: "b%dh%d-%dm%dn%dd%dw%ds%d" % s)
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_backward_of_groups_and_sinks(shape, dtype):
+    _check(shape, dtype)
+
+
 @pytest.mark.parametrize("scale", [0.3, 0.0, -0.1])
 def test_scales(scale):
     """(0 and below: the CUDA-core kernels)"""
