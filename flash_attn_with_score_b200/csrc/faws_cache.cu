@@ -644,6 +644,10 @@ __global__ void __launch_bounds__(CTA_THREADS, CTAS_PER_SM) cache_attn_kernel(co
     const int g = lane >> 2, t = lane & 3;
     const int krow = (g & 1) ? ((g >> 1) ^ 1) + 4 : g >> 1;      // token_of(g); token_of(i + 8) = token_of(i) + 8
     const int tok[4] = {t, (t ^ 1) + 4, t + 8, (t ^ 1) + 12};    // token_of(2 t), (2 t + 1), (2 t + 8), (2 t + 9)
+    // -8 in every place, kept in registers: as a constant it is put there again for each product
+    uint32_t less8[4];
+    asm volatile("mov.b32 %0, 0x80208020;\n\tmov.b32 %1, 0x82008200;\n\tmov.b32 %2, 0x80208020;\n\tmov.b32 %3, 0x82008200;"
+                 : "=r"(less8[0]), "=r"(less8[1]), "=r"(less8[2]), "=r"(less8[3]));
     float* so = reinterpret_cast<float*>(smem + L::out_off) + warp * RT * L::kOutRow;
     float4* table = reinterpret_cast<float4*>(so);  // [keys, values][pair of groups][token]
     float2* ml = reinterpret_cast<float2*>(smem + L::ml_off);
@@ -923,7 +927,6 @@ __global__ void __launch_bounds__(CTA_THREADS, CTAS_PER_SM) cache_attn_kernel(co
               x23 <<= 2;
             }
             const uint32_t a0[4] = {x01 & kLow, x01 & kHigh, x23 & kLow, x23 & kHigh};
-            const uint32_t less8[4] = {0x80208020u, 0x82008200u, 0x80208020u, 0x82008200u};  // -8 in every place
             [[maybe_unused]] uint32_t a1[4];
             if constexpr (MT == 2) {
               const uint32_t y01 = __byte_perm(vw[0][gi >> 1], vw[1][gi >> 1], swapped);
