@@ -475,5 +475,6 @@ def launch_count() -> int:
 
 
 def device_status(reset: bool = True) -> int:
-    """Synchronise and read the give-up flag of the tcgen05 kernels' bounded waits (0 = clean)."""
+    """Synchronise and read the device's status word: 0 = clean, bit 0: a kernel's bounded wait gave up (its outputs are
+    invalid), bit 1: a cache operator was given a page or a length that the cache does not have."""
     return int(_lib.load().faws_device_status(1 if reset else 0))

@@ -139,7 +139,8 @@ def attention_with_kv_cache(q, cache, page_table, lengths, window=None, sinks=0,
         p = _lib.Problem(B=B, Hq=H, Hk=cache.heads, M=M, N=1, D=D, dtype=_DTYPES[q.dtype], causal=1,
                          sm_scale=float(1.0 / math.sqrt(D) if sm_scale is None else sm_scale), m_begin=0, m_end=M,
                          q=_tensor(q), out=_tensor(out), log_normalizer=L.data_ptr() if L is not None else None)
-        n = _lib.load().faws_kv_cache_workspace_bytes(C.byref(p))
+        with torch.cuda.device(cache.device):  # (as many shares as that device has room for)
+            n = _lib.load().faws_kv_cache_workspace_bytes(C.byref(p))
         ws = torch.empty(n, device=q.device, dtype=torch.uint8)
         _run(cache, "faws_attention_with_kv_cache", C.byref(p), C.byref(cache._struct), C.byref(batch),
              window, sinks, C.c_void_p(ws.data_ptr()), n)
