@@ -667,7 +667,7 @@ tc_fwd_kernel(const __grid_constant__ TcMaps maps, const FwdParams p, const __gr
     constexpr bool store_scores16 = HOOK == kHookScores16;
     const float masked_f = __uint_as_float(p.masked_bits);
     // per item
-    int r_tile, i, qb128;  // first row of the query tile, this thread's row
+    int r_tile, i, my_nt, qb128;  // first row of the query tile, this thread's row, end of its key-tile range
     int vis_end;                  // causal: this thread's row sees the keys before it
     bool row_ok, part_on;
     uint32_t drop_row;  // Philox counter of (b, h, i, key 0) without the call's offset, 32-bit wrap-around
@@ -1127,6 +1127,7 @@ tc_fwd_kernel(const __grid_constant__ TcMaps maps, const FwdParams p, const __gr
     for (int k = 0;; ++k) {
     r_tile = r_tile_of[qt];
     i = r_tile + row;
+    my_nt = nt_q[qt];
     vis_end = (pack_m > 0 ? i % pack_m : i) + p.p_seq + 1;
     row_ok = i >= p.m_begin && i < p.m_end;
     qb128 = r_tile / BM;
@@ -1140,7 +1141,7 @@ tc_fwd_kernel(const __grid_constant__ TcMaps maps, const FwdParams p, const __gr
       int cnt = 0;
       for (int it = 0; it < nt; ++it) {
         const int tk = tile_of(it);
-        if (SPLIT ? ((it & 1) != qt) : !visits(qt, tk)) continue;
+        if (SPLIT ? ((it & 1) != qt) : WIN ? !visits(qt, tk) : (tk >= my_nt)) continue;
         const int n0 = tk * BN;
         [[maybe_unused]] uint4* mask_row = nullptr;
         if constexpr (DROP == kReadMask || DROP == kKeepMask)
@@ -1159,7 +1160,7 @@ tc_fwd_kernel(const __grid_constant__ TcMaps maps, const FwdParams p, const __gr
     const float rs = rs_raw * scale;
 
     // ---- epilogue: O / l -> out, log-normaliser, row sums, masked fill of unvisited tiles
-    if (alive && visits_any(qt)) {
+    if (alive && (WIN ? visits_any(qt) : my_nt > kt0)) {
       if (!mbar_wait(&bars->o_done[qt], o_cnt & 1, abort_flag)) alive = false;
       ++o_cnt;
       tc_fence_after();
@@ -1191,7 +1192,7 @@ tc_fwd_kernel(const __grid_constant__ TcMaps maps, const FwdParams p, const __gr
     if (write_out) {
       float inv = l_all > 0.f ? 1.f / l_all : 0.f;
       if constexpr (DROP != kNoDrop) inv *= p.drop.out_scale;
-      if (visits_any(qt)) {
+      if (WIN ? visits_any(qt) : my_nt > kt0) {
         // Each warp stages its 32 x D output block (128B-swizzled) and stores it with TMA: in its own
         // staging block where the hook leaves that free, so that a persistent CTA's next Q tiles can land
         // meanwhile; in the Q tiles' shared memory (every MMA of the CTA has completed) under the hooks
