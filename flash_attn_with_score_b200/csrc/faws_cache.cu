@@ -553,13 +553,20 @@ __global__ void __launch_bounds__(CTA_THREADS, CTAS_PER_SM) cache_attn_kernel(co
       bars->walk = first;
       bars->shares = shares;
     }
-  } else if (warp == 1) {  // sequences without a key have no tiles: their rows are zero
-    for (int b = blockIdx.x; b < p.batch.B; b += gridDim.x) {
+  } else if (warp == 1) {
+    // Sequences without a key have no tiles: their rows are zero.  A sequence's rows are shared by as many CTAs as leave each 64
+    // stores of a warp, one where a sequence has few rows (two sequences of 2048 rows, 32 heads of 128, one of them empty: 11.7 ms
+    // with one CTA for it).
+    constexpr int kLanes = D / 4, kRows = 32 / kLanes;  // lanes of a row, rows of a warp
+    const int parts = (int)min((int64_t)gridDim.x, ((int64_t)p.cache.Hk * p.rows + 64 * kRows - 1) / (64 * kRows));
+    for (int64_t y = blockIdx.x; y < (int64_t)p.batch.B * parts; y += gridDim.x) {
+      const int b = (int)(y / parts), part = (int)(y - (int64_t)b * parts);
       bool bad = false;
       if (span_of(p, b, &bad).nt > 0) continue;
-      for (int x = lane; x < p.cache.Hk * p.rows * (D / 4); x += 32) {
-        const int row = x / (D / 4), hk = row / p.rows;
-        store_row<T>(p, b, hk, row - hk * p.rows, (x % (D / 4)) * 4, make_float4(0.f, 0.f, 0.f, 0.f), 0.f, 0.f);
+      for (int hk = 0, r = part * kRows + lane / kLanes;; r += parts * kRows) {
+        for (; r >= p.rows && hk < p.cache.Hk; ++hk) r -= p.rows;
+        if (hk >= p.cache.Hk) break;
+        store_row<T>(p, b, hk, r, lane % kLanes * 4, make_float4(0.f, 0.f, 0.f, 0.f), 0.f, 0.f);
       }
     }
   }

@@ -197,6 +197,21 @@ def test_values_all_of_one_size(size):
     _check(s, 4, 1)
 
 
+@pytest.mark.parametrize("Hq,Hk,M,D", [(4, 4, 1, 64), (6, 2, 300, 16), (3, 1, 1001, 128), (32, 8, 700, 32)])
+def test_empty_sequences_of_any_number_of_rows(Hq, Hk, M, D):
+    """Zeros and -inf in every row of them, whatever lay in the memory of the outputs."""
+    import flash_attn_with_score_b200 as F
+    s = Setup([0, 30, 0, 1, 0], Hk, D, F16, 16)
+    poison = [torch.full((5, Hq, M, *d), float("nan"), dtype=t, device="cuda") for d, t in (((D,), F16), ((), torch.float32))]
+    del poison
+    q = torch.randn((5, Hq, M, D), generator=torch.Generator().manual_seed(1)).half().cuda()
+    for _ in range(4):
+        out, L = F.attention_with_kv_cache(q, s.cache, s.table, s.lengths, return_log_normalizer=True)
+        assert bool((out[::2] == 0).all()) and bool((L[::2] == -float("inf")).all())
+        out.fill_(float("nan")), L.fill_(float("nan"))
+    _check(s, Hq, M)
+
+
 def test_unwritten_rows_of_a_page_do_not_matter():
     import flash_attn_with_score_b200 as F
     s = Setup([130, 40], 2, 128, F16, 64)
