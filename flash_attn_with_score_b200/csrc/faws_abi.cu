@@ -502,8 +502,8 @@ int validate_cache(const faws_kv_cache* c, const faws_cache_batch* b, int64_t ro
   if (b->page_table == nullptr || b->lengths == nullptr || b->table_stride < 0) return FAWS_EINVAL;
   for (const void* x : {c->k_codes, c->v_codes, c->k_scales, c->v_scales})
     if (x == nullptr || reinterpret_cast<uintptr_t>(x) % 16 != 0) return FAWS_EINVAL;
-  // a block has 2048 elements of these rows, a grid 2^31 - 1 blocks
-  if ((int64_t)b->B * c->Hk > (int64_t(1) << 40) / (rows * c->D)) return FAWS_EINVAL;
+  // rows are counted in 32 bits together with positions; a block has 2048 elements of these rows, a grid 2^31 - 1 blocks
+  if (rows > (1 << 30) || (int64_t)b->B * c->Hk > (int64_t(1) << 40) / (rows * c->D)) return FAWS_EINVAL;
   return FAWS_OK;
 }
 CacheParams make_cache(const faws_kv_cache* c) {
@@ -894,7 +894,7 @@ int faws_attention_with_kv_cache(const faws_problem* p, const faws_kv_cache* c, 
   const int st = validate_cache(c, batch, rows);
   if (st != FAWS_OK) return st;
   if (p->B != batch->B || p->Hk != c->Hk || p->D != c->D || p->dtype != c->dtype) return FAWS_EINVAL;
-  if (p->q.ptr == nullptr || p->out.ptr == nullptr || window < 0 || sinks < 0 || rows > (1 << 30)) return FAWS_EINVAL;
+  if (p->q.ptr == nullptr || p->out.ptr == nullptr || window < 0 || sinks < 0) return FAWS_EINVAL;
   // the kernel counts tiles of 128 tokens in 32 bits
   const int64_t tiles = ((int64_t)batch->max_pages * c->page_size + 127) / 128;
   if (tiles * ((rows + 7) / 8) > ((int64_t(1) << 31) - 1) / ((int64_t)p->B * p->Hk)) return FAWS_EINVAL;

@@ -339,7 +339,8 @@ typedef struct faws_kv_cache {
 /*
  * The sequences of a call.  Position n of sequence b lies in page page_table[b * table_stride + n / page_size].  lengths[b]
  * counts the tokens of sequence b, those of the call among them: the calls below take `rows` (M) rows per sequence, row m
- * being position lengths[b] - rows + m (aligned to the end, as causal masks are).  Rows before position 0 are padding.
+ * being position lengths[b] - rows + m (aligned to the end, as causal masks are).  Rows before position 0 are padding.  A head
+ * has at most 2^30 rows of a sequence (of attention: a kv head, over the query heads that share it).
  * Both arrays are on the device.  A length below 0 or beyond max_pages * page_size is taken as the nearest bound and a
  * page outside [0, pages) is not touched; both raise the device's status word (faws_device_status: 2).
  */

@@ -73,6 +73,20 @@ def test_bad_rows_and_attention_arguments(lib):
     assert call(q) == -1
 
 
+def test_more_rows_than_are_counted(lib):
+    """B 1, two heads: 2^30 rows are the most, and the elements of a call's grid are bounded."""
+    from flash_attn_with_score_b200 import _lib
+    cache, batch, p = _structs(B=1, D=16)
+    p.B, p.D = 1, 16
+    t = _lib.Tensor(4096, 0, 0, 0)
+    for rows in (2 ** 30 + 1, 2 ** 31 - 1):
+        for fn in (lib.faws_kv_cache_write, lib.faws_kv_cache_read):
+            assert fn(C.byref(cache), C.byref(batch), C.byref(t), C.byref(t), rows, None) == -1
+        p.M = p.m_end = rows
+        p.Hq = 2
+        assert lib.faws_attention_with_kv_cache(C.byref(p), C.byref(cache), C.byref(batch), 0, 0, 4096, 1 << 30, None) == -1
+
+
 def test_python_refusals():
     import flash_attn_with_score_b200 as F
     with pytest.raises(RuntimeError, match="CUDA"):
