@@ -261,6 +261,8 @@ class _WindowFunction(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, do, *ignored):
+        if torch.is_grad_enabled():
+            raise RuntimeError("attention_with_window has no second derivative (create_graph)")
         q, k, v, o, L = ctx.saved_tensors
         if do is None:
             return (*map(torch.zeros_like, (q, k, v)), *(None,) * 5)
@@ -276,7 +278,7 @@ class _WindowFunction(torch.autograd.Function):
 
 def attention_with_window(q, k, v, window, sinks=0, sm_scale=None, return_log_normalizer=False,
                           *, backend=None, kv_splits=None):
-    """Causal attention to a bounded context, differentiable in q, k, v: a query sees the last ``window`` keys up to its own
+    """Causal attention to a bounded context, differentiable once in q, k, v: a query sees the last ``window`` keys up to its own
     position (bottom-right aligned, as everywhere) and the first ``sinks`` keys of the sequence; rows that see none are zero.
     Hidden keys and values must be finite, as in ``attention``: a weight of zero times an infinity is not zero.
 

@@ -116,6 +116,7 @@ struct WindowFunction : public torch::autograd::Function<WindowFunction> {
     return {out, L};
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    TORCH_CHECK(!at::GradMode::is_enabled(), "attention_with_window has no second derivative (create_graph)");
     const auto saved = ctx->get_saved_variables();
     const at::Tensor &q = saved[0], &k = saved[1], &v = saved[2], &out = saved[3], &L = saved[4];
     const at::Tensor none;

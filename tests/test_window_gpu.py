@@ -303,6 +303,39 @@ def test_together_window_prefill_then_cache():
     assert F.device_status() == 0
 
 
+@pytest.mark.parametrize("kv_splits", [None, 1])
+def test_no_second_derivative(kv_splits):
+    """Refused, where a gradient without a graph would drop terms silently."""
+    import flash_attn_with_score_b200 as F
+    q = torch.randn((1, 2, 40, 64), device="cuda").half().requires_grad_()
+    out = F.attention_with_window(q, q, q, 10, kv_splits=kv_splits).float().sum()
+    with pytest.raises(RuntimeError, match="second derivative"):
+        torch.autograd.grad(out, q, create_graph=True, retain_graph=True)
+    want, = torch.autograd.grad(out, q)
+    y = torch.utils.checkpoint.checkpoint(lambda x: F.attention_with_window(x, x, x, 10, kv_splits=kv_splits), q, use_reentrant=False)
+    assert torch.equal(torch.autograd.grad(y.float().sum(), q)[0], want)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_expanded_inputs(D):
+    """Heads, sequences and rows that are one in memory, and their gradients: the sums over what shares them."""
+    import flash_attn_with_score_b200 as F
+    B, H, N = 2, 4, 300
+    g = torch.Generator().manual_seed(5)
+    make = lambda *s: torch.randn(s, generator=g).half().cuda()  # noqa: E731
+    q, do = make(B, H, N, D), make(B, H, N, D)
+    for shape in ((B, 1, N, D), (1, H, N, D), (1, 1, N, D), (B, H, 1, D)):
+        k, v = make(*shape), make(*shape)
+        grads = []
+        for whole in (False, True):
+            xs = [x.clone().requires_grad_() for x in (q, k, v)]
+            wide = [x.expand(B, H, N, D) for x in xs]
+            out = F.attention_with_window(*([x.contiguous() for x in wide] if whole else wide), 64, 3)
+            grads.append((out, *torch.autograd.grad(out, wide, do)))
+        for a, b in zip(*grads):
+            assert torch.equal(a, b)
+
+
 def test_refusals():
     import flash_attn_with_score_b200 as F
     q, k, v, _ = _inputs(1, 4, 2, 64, 64, 64, F16)
