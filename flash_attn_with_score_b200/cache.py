@@ -27,7 +27,7 @@ class KVCache4:
     A row of a head is held in groups of min(32, head_dim) neighbouring elements: a scale bf16(amax / 7) and codes from -7 to
     7, halves rounded away from zero.  A group that holds an infinity or a NaN reads as NaN.  ``k_codes``, ``v_codes`` (pages,
     heads, page_size, head_dim / 2) uint8 and ``k_scales``, ``v_scales`` (pages, heads, page_size, groups) bfloat16 may be copied
-    page by page; how codes lie within a row is the library's affair."""
+    page by page; how codes lie within a row is the library's affair.  The tensors themselves are the cache's for good."""
 
     def __init__(self, pages, page_size, heads, head_dim, dtype=torch.float16, device="cuda"):
         if dtype not in _DTYPES:
@@ -47,6 +47,11 @@ class KVCache4:
         self._struct = _lib.KVCache(self.k_codes.data_ptr(), self.v_codes.data_ptr(), self.k_scales.data_ptr(),
                                     self.v_scales.data_ptr(), pages, page_size, heads, head_dim, _DTYPES[dtype])
         self._plain = (C.addressof(self._struct), self.device.index)
+
+    def __setattr__(self, name, value):
+        if name in self.__dict__:  # (calls go by what the cache was made with)
+            raise AttributeError(f"a cache's {name} cannot be replaced: copy into its tensors, or make another cache")
+        super().__setattr__(name, value)
 
 
 def _batch(cache, page_table, lengths, B):

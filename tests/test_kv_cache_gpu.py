@@ -365,6 +365,17 @@ def test_graph_stream_and_two_at_once():
     assert F.device_status() == 0
 
 
+def test_a_cache_stays_what_it_is():
+    import copy
+    s = Setup([64], 2, 64, F16, 16)
+    for name in ("k_codes", "v_codes", "k_scales", "v_scales", "pages", "page_size", "heads", "head_dim", "dtype"):
+        with pytest.raises(AttributeError, match=name):
+            setattr(s.cache, name, getattr(s.cache, name))
+    with pytest.raises(ValueError):  # two caches that say to be apart and share their memory
+        copy.deepcopy(s.cache)
+    _check(s, 4, 1)
+
+
 def test_refusals():
     import flash_attn_with_score_b200 as F
     s = Setup([64], 2, 64, F16, 16)
