@@ -6,8 +6,9 @@ sequence.  ``lengths[b]`` counts the tokens of sequence b, those of the call amo
 Both are int32 tensors on the cache's device, so that a decoding step can be captured in a graph and replayed with
 others in place.
 
-Positions, pages and lengths are known to the device alone.  What does not exist there is never touched: a page outside the
-cache is not written and reads as NaN, a length beyond the table is taken as the table's; ``device_status()`` then has bit 1 set.
+Positions, pages and lengths are known to the device alone.  What does not exist there is never touched: rows on a page outside
+the cache, or at a position behind the table's last page, are not written and read as NaN, as do outputs that see such keys (a
+row at such a position sees its own); a length below 0 is taken as 0.  ``device_status()`` then has bit 1 set.
 """
 from __future__ import annotations
 

@@ -87,13 +87,17 @@ __device__ __forceinline__ float fast_log2(float x) {
   return y;
 }
 
-// Length of sequence b as the cache can hold it; *bad where lengths says otherwise.
-__device__ __forceinline__ int cached_length(const CacheBatch& c, int page_shift, int b, bool* bad) {
+// Positions that a sequence's row of the table has room for.  Those behind them do not exist: rows are not written there and read as
+// NaN, keys are NaN.
+__device__ __forceinline__ int table_room(const CacheBatch& c, int page_shift) {
+  const long long room = (long long)c.max_pages << page_shift;
+  return room > 0x3fffffff ? 0x3fffffff : (int)room;
+}
+// Length of sequence b, 0 where `lengths` says less; *bad where it says less or more than `room`.
+__device__ __forceinline__ int told_length(const CacheBatch& c, int room, int b, bool* bad) {
   const int n = c.lengths[b];
-  const long long cap = (long long)c.max_pages << page_shift;
-  const int most = cap > 0x3fffffff ? 0x3fffffff : (int)cap;
-  if (n < 0 || n > most) *bad = true;
-  return max(0, min(n, most));
+  if (n < 0 || n > room) *bad = true;
+  return max(0, n);
 }
 
 // ---------------------------------------------------------------------------------------------- write, read
@@ -116,10 +120,11 @@ constexpr int kRowsEach = 4;
 struct RowPlace {
   const int32_t* table;
   int first;           // position of row 0
+  int stop;            // the rows from here on lie behind the table, or do not belong to the call
   int shift, pages, Hk, hk;
   int one;             // the page of all rows, or kSeveral
   static constexpr int kSeveral = -0x7fffffff;
-  __device__ __forceinline__ bool real(int m, int rows) const { return m < rows && first + m >= 0; }
+  __device__ __forceinline__ bool real(int m) const { return m < stop && first + m >= 0; }
   __device__ __forceinline__ int64_t at(int m, bool* bad) const {
     const int pos = first + m, page = one != kSeveral ? one : table[pos >> shift];
     if ((unsigned)page >= (unsigned)pages) {
@@ -134,13 +139,15 @@ __device__ __forceinline__ RowPlace row_place(const CacheParams& c, const CacheB
                                               bool* bad) {
   RowPlace p;
   p.table = bt.table + (int64_t)b * bt.table_stride;
-  p.first = cached_length(bt, c.page_shift, b, bad) - rows;
+  const int room = table_room(bt, c.page_shift);
+  p.first = told_length(bt, room, b, bad) - rows;
+  p.stop = min(rows, room - p.first);
   p.shift = c.page_shift;
   p.pages = c.pages;
   p.Hk = c.Hk;
   p.hk = hk;
-  const int lo = max(p.first + m0, 0) >> c.page_shift, hi = (p.first + min(m1, rows) - 1) >> c.page_shift;
-  p.one = lo == hi ? p.table[lo] : RowPlace::kSeveral;  // (hi < 0: no row is real)
+  const int lo = max(p.first + m0, 0) >> c.page_shift, hi = (p.first + min(m1, p.stop) - 1) >> c.page_shift;
+  p.one = lo == hi ? p.table[lo] : RowPlace::kSeveral;  // (hi < 0, or before lo: no row is real)
   return p;
 }
 
@@ -185,7 +192,7 @@ __device__ __forceinline__ void write_rows(const CacheParams& c, const CacheRows
 #pragma unroll
   for (int y = 0; y < EACH; ++y) {
     in[y] = make_uint4(0u, 0u, 0u, 0u);
-    if (WHOLE || place.real(m0 + y * lanes, r.rows)) {
+    if (WHOLE || place.real(m0 + y * lanes)) {
       const T* from = src + y * lanes * ss;
       if (WHOLE || r.vec) in[y] = *reinterpret_cast<const uint4*>(from);
       else {
@@ -229,7 +236,7 @@ __device__ __forceinline__ void write_rows(const CacheParams& c, const CacheRows
     for (int e = 6; e >= 0; --e) word = word * 16u + __float_as_uint(fmaf(x[e], inv, 8388616.f));
     word -= 0xfb000000u;  // what is left of 2^23, 0x4b000000 in elements 0 and 1
     if (D >= 32) word = VALUES ? exchange_halves<D>(rotate_halves(word), w, true) : __funnelshift_l(word, word, 2);
-    if (WHOLE || place.real(m, r.rows)) {
+    if (WHOLE || place.real(m)) {
       const int64_t row = WHOLE ? row0 + y * lanes : place.at(m, bad);
       if (WHOLE || row >= 0) {
         *reinterpret_cast<uint32_t*>(codes + row * (D / 2)) = word;
@@ -254,7 +261,7 @@ __device__ __forceinline__ void read_rows(const CacheParams& c, const CacheRows&
     const int m = m0 + y * lanes;
     words[y] = D >= 32 ? 0x22222222u : 0x88888888u;  // padding: zeros
     sbits[y] = 0u;
-    if (WHOLE || place.real(m, r.rows)) {
+    if (WHOLE || place.real(m)) {
       const int64_t row = WHOLE ? row0 + y * lanes : place.at(m, bad);
       sbits[y] = 0xffc0u;
       if (WHOLE || row >= 0) {
@@ -285,6 +292,17 @@ __device__ __forceinline__ void read_rows(const CacheParams& c, const CacheRows&
       }
     }
   }
+  // Rows behind the table, zeros so far.  (Told apart where words are fetched they cost every call: 3 x 1531 rows of 12 heads of 64,
+  // fp16, pages of 16: 6.8 us, 5.6 so.)
+  if (!WHOLE && place.stop < r.rows) {
+#pragma unroll 1
+    for (int y = 0; y < EACH; ++y) {
+      const int m = m0 + y * lanes;
+      if (m < place.stop || m >= r.rows) continue;
+#pragma unroll 1
+      for (int e = 0; e < 8; ++e) reinterpret_cast<uint16_t*>(dst + y * lanes * ss)[e] = 0x7fffu;
+    }
+  }
 }
 
 // Keys in the first half of the grid, values in the second.  CTAs whose rows all exist, on one page, with 16-byte accesses, go
@@ -303,7 +321,7 @@ __global__ void __launch_bounds__(256) cache_rows_kernel(const CacheParams c, co
   t.first = (blockIdx.x - bh * r.tiles) * rows;
   bool bad = false;
   const RowPlace place = row_place(c, bt, r.rows, t.b, t.hk, t.first, t.first + rows, &bad);
-  const bool whole = r.vec && t.first + rows <= r.rows && place.first + t.first >= 0 && (unsigned)place.one < (unsigned)c.pages;
+  const bool whole = r.vec && t.first + rows <= place.stop && place.first + t.first >= 0 && (unsigned)place.one < (unsigned)c.pages;
   auto run = [&](auto values, auto all) {
     if constexpr (WRITE) write_rows<T, D, decltype(values)::value, decltype(all)::value, EACH>(c, r, place, t, &bad);
     else read_rows<T, D, decltype(values)::value, decltype(all)::value, EACH>(c, r, place, t, &bad);
@@ -381,15 +399,22 @@ __device__ __forceinline__ bool consumers_any(bool mine) {
   return any != 0;
 }
 
-// Tiles that the rows of a sequence see: [0, ns), then [w0, w0 + nt - ns).
+// Tokens of sequence b that the table has no room for.  (Read where it is wanted: kept, it would be spilled.)
+__device__ __forceinline__ int tokens_beyond(const CacheAttnParams& p, int b) {
+  return max(0, p.batch.lengths[b] - table_room(p.batch, p.cache.page_shift));
+}
+// Tiles that the rows of a sequence see: [0, ns), then [w0, w0 + nt - ns).  `len`: the tokens that the table has room for.
 struct Span {
   int len, lo, ns, w0, nt;
   __device__ __forceinline__ int tile(int it) const { return it < ns ? it : w0 + it - ns; }
 };
 __device__ __forceinline__ Span span_of(const CacheAttnParams& p, int b, bool* bad) {
   Span s;
-  s.len = cached_length(p.batch, p.cache.page_shift, b, bad);
-  s.lo = max(0, s.len - p.M - p.window + 1);  // the first key that the first row's window has
+  const int room = table_room(p.batch, p.cache.page_shift);
+  const int end = told_length(p.batch, room, b, bad);
+  s.len = min(end, room);
+  // the first key that the first row's window has (the last one where there is none: a sequence with keys has a tile)
+  s.lo = max(0, min(end - p.M - p.window + 1, s.len - 1));
   s.w0 = s.lo / TT;
   s.ns = min((min(p.sinks, s.len) + TT - 1) / TT, s.w0);
   s.nt = s.len > 0 ? s.ns + (s.len + TT - 1) / TT - s.w0 : 0;
@@ -506,11 +531,14 @@ __device__ __forceinline__ float* part_slot(const CacheAttnParams& p, int share,
 }
 __device__ __forceinline__ int4* part_header(const CacheAttnParams& p, int share) { return reinterpret_cast<int4*>(p.parts) + share; }
 
-// Four elements of a finished row: sum / den, zeros for a row that saw nothing.
+// Four elements of a finished row: sum / den, zeros for a row that saw nothing, NaN for the last `beyond` rows of a head, whose
+// own keys lie behind the table.
 template <typename T>
-__device__ __forceinline__ void store_row(const CacheAttnParams& p, int b, int hk, int r, int d, float4 sum, float top, float den) {
+__device__ __forceinline__ void store_row(const CacheAttnParams& p, int b, int beyond, int hk, int r, int d, float4 sum, float top,
+                                          float den) {
   if (r >= p.rows) return;
   const int head = hk * p.G + r / p.M, i = r % p.M;
+  if (i >= p.M - beyond) den = __int_as_float(0x7fffffff);
   const float inv = den == 0.f ? 0.f : 1.f / den;  // (a NaN stays one)
   T* dst = static_cast<T*>(p.out) + b * p.o_sb + (int64_t)head * p.o_sh + (int64_t)i * p.o_ss + d;
   const uint32_t lo = pack2<T>(sum.x * inv, sum.y * inv), hi = pack2<T>(sum.z * inv, sum.w * inv);
@@ -566,7 +594,7 @@ __global__ void __launch_bounds__(CTA_THREADS, CTAS_PER_SM) cache_attn_kernel(co
       for (int hk = 0, r = part * kRows + lane / kLanes;; r += parts * kRows) {
         for (; r >= p.rows && hk < p.cache.Hk; ++hk) r -= p.rows;
         if (hk >= p.cache.Hk) break;
-        store_row<T>(p, b, hk, r, lane % kLanes * 4, make_float4(0.f, 0.f, 0.f, 0.f), 0.f, 0.f);
+        store_row<T>(p, b, 0, hk, r, lane % kLanes * 4, make_float4(0.f, 0.f, 0.f, 0.f), 0.f, 0.f);
       }
     }
   }
@@ -662,6 +690,7 @@ __global__ void __launch_bounds__(CTA_THREADS, CTAS_PER_SM) cache_attn_kernel(co
     bool ok = true;
     do {
       const int hk = w.item / p.row_blocks, r0 = (w.item % p.row_blocks) * RT, cnt = w.count();
+      const int end = w.span.len + tokens_beyond(p, w.b);  // one behind the last row's position
       // ---- the rows' queries as fp16 operands, and -8 sum of each group; a lane loads row g of 8
       uint32_t q[NB][NG][2][2];
       uint64_t qbias[NB][NG];    // of rows 2 t and 2 t + 1, as f
@@ -691,7 +720,7 @@ __global__ void __launch_bounds__(CTA_THREADS, CTAS_PER_SM) cache_attn_kernel(co
         const float mul = __int_as_float((127 + k) << 23);
         // 2^22 undoes the subnormal; in two factors, so that neither leaves fp32's range
         const float my_f = p.sm_scale * kLog2e * __int_as_float((127 + 22) << 23) * __int_as_float((127 - k) << 23);
-        const int my_hi = real ? w.span.len - p.M + i + 1 : 0;
+        const int my_hi = real ? end - p.M + i + 1 : 0;
         // rows 2 t and 2 t + 1 are loaded by the lanes 8 t and 8 t + 4
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
@@ -733,7 +762,8 @@ __global__ void __launch_bounds__(CTA_THREADS, CTAS_PER_SM) cache_attn_kernel(co
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) o[nb][gi][mt][c] = 0.f;
       }
-      const int hi_first = w.span.len - p.M + 1, lo_last = w.span.len - p.window;  // of the first, the last row
+      // of the first, the last row (rows whose own key is behind `len` become NaN, whatever they take part in)
+      const int hi_first = end - p.M + 1, lo_last = end - p.window;
 
       // ---- 32 tokens from `base` of the stage on, the first of them at position n0, in two parts of 16; their scores come first, so
       // that the maximum is looked at once
@@ -1005,7 +1035,7 @@ __global__ void __launch_bounds__(CTA_THREADS, CTAS_PER_SM) cache_attn_kernel(co
           sum.x = fmaf(e, v.x, sum.x); sum.y = fmaf(e, v.y, sum.y); sum.z = fmaf(e, v.z, sum.z); sum.w = fmaf(e, v.w, sum.w);
         }
         if (begins && ends) {
-          store_row<T>(p, w.b, hk, r0 + row, d, sum, top, den);
+          store_row<T>(p, w.b, tokens_beyond(p, w.b), hk, r0 + row, d, sum, top, den);
         } else {
           float* part = part_slot<D>(p, blockIdx.x, begins ? 1 : 0) + row * (D + 4);
           *reinterpret_cast<float4*>(part + d) = sum;
@@ -1069,7 +1099,7 @@ __global__ void __launch_bounds__(256) cache_combine_kernel(const CacheAttnParam
         sum.z = fmaf(e, v[y].z, sum.z); sum.w = fmaf(e, v[y].w, sum.w);
       }
     }
-    store_row<T>(p, head.x, hk, r0 + row, d, sum, top, den);
+    store_row<T>(p, head.x, tokens_beyond(p, head.x), hk, r0 + row, d, sum, top, den);
   }
 }
 

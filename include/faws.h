@@ -341,8 +341,9 @@ typedef struct faws_kv_cache {
  * counts the tokens of sequence b, those of the call among them: the calls below take `rows` (M) rows per sequence, row m
  * being position lengths[b] - rows + m (aligned to the end, as causal masks are).  Rows before position 0 are padding.  A head
  * has at most 2^30 rows of a sequence (of attention: a kv head, over the query heads that share it).
- * Both arrays are on the device.  A length below 0 or beyond max_pages * page_size is taken as the nearest bound and a
- * page outside [0, pages) is not touched; both raise the device's status word (faws_device_status: 2).
+ * Both arrays are on the device.  A length below 0 is taken as 0.  Positions from max_pages * page_size on (2^30 - 1 at most)
+ * do not exist, nor do those on a page outside [0, pages): they are not touched.  A length below 0 or with such positions and a
+ * page out of range raise the device's status word (faws_device_status: 2).
  */
 typedef struct faws_cache_batch {
   const int32_t* page_table;
@@ -351,12 +352,13 @@ typedef struct faws_cache_batch {
   int32_t B, max_pages;
 } faws_cache_batch;
 
-/* Quantises the rows of k and v, (B,Hk,rows,D) views, into the cache; padding rows and rows on bad pages are skipped.  The
- * positions that a call writes are to be in different places: two rows for the same place leave it undefined. */
+/* Quantises the rows of k and v, (B,Hk,rows,D) views, into the cache; padding rows and rows at positions that do not exist are
+ * skipped.  The positions that a call writes are to be in different places: two rows for the same place leave it undefined. */
 int faws_kv_cache_write(const faws_kv_cache* c, const faws_cache_batch* batch, const faws_tensor* k, const faws_tensor* v,
                         int32_t rows, void* stream);
 
-/* The values of rows of the cache, into k and v, (B,Hk,rows,D) views; padding rows become 0, rows on bad pages NaN. */
+/* The values of rows of the cache, into k and v, (B,Hk,rows,D) views; padding rows become 0, rows at positions
+ * that do not exist NaN. */
 int faws_kv_cache_read(const faws_kv_cache* c, const faws_cache_batch* batch, const faws_tensor* k, const faws_tensor* v,
                        int32_t rows, void* stream);
 
@@ -364,7 +366,7 @@ int faws_kv_cache_read(const faws_kv_cache* c, const faws_cache_batch* batch, co
  * Causal attention of the last p->M rows of each sequence over the cache.  Of p: B, Hq, Hk, M, D, dtype, sm_scale, q, out and
  * log_normalizer ((B,Hq,M) or NULL) are used; the rest is ignored.  window 0: a row sees every key up to its own position;
  * window > 0: the last `window` of those, and the first `sinks` ones (faws_attention_with_window).  Rows that see nothing (padding, empty
- * sequences) become 0.  Keys on bad pages are NaN.  Deterministic.  Workspace: faws_kv_cache_workspace_bytes(p), 256-byte
+ * sequences) become 0.  Keys at positions that do not exist are NaN, and with them the rows there.  Deterministic.  Workspace: faws_kv_cache_workspace_bytes(p), 256-byte
  * aligned.
  */
 int faws_attention_with_kv_cache(const faws_problem* p, const faws_kv_cache* c, const faws_cache_batch* batch,
