@@ -326,7 +326,7 @@ tc_colsoftmax_kernel(const __grid_constant__ CsMaps maps, const ColSoftmaxParams
     }
   }
   if (*abort_flag) {
-    if (threadIdx.x == 0 && status != nullptr) atomicExch(status, 1);
+    if (threadIdx.x == 0 && status != nullptr) atomicOr(status, 1);
     for (int w = 0; w < 50; ++w) __nanosleep(20000);
     __syncthreads();
   }
@@ -473,7 +473,7 @@ __global__ void wait_give_up_kernel(int* __restrict__ status, long long limit_cy
   __syncthreads();
   if (threadIdx.x == 0) mbar_wait(&bar, 0, &abort_flag, limit_cycles);
   __syncthreads();
-  if (abort_flag != 0 && threadIdx.x == 0 && status != nullptr) atomicExch(status, 1);
+  if (abort_flag != 0 && threadIdx.x == 0 && status != nullptr) atomicOr(status, 1);
 }
 }  // namespace
 

@@ -206,7 +206,7 @@ tc_bwd_kernel(const __grid_constant__ BwMaps maps, const BwTcParams p, int* __re
   volatile int* abort_flag = &bars->abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (smem_u32(smem) & 1023u) {  // 128-byte swizzle atoms are 1 KB; the full shared memory leaves no slack to align by
-    if (threadIdx.x == 0 && status != nullptr) atomicExch(status, 1);
+    if (threadIdx.x == 0 && status != nullptr) atomicOr(status, 1);
     return;
   }
 
@@ -785,7 +785,7 @@ tc_bwd_kernel(const __grid_constant__ BwMaps maps, const BwTcParams p, int* __re
   tc_fence_before();
   __syncthreads();
   if (*abort_flag) {
-    if (threadIdx.x == 0 && status != nullptr) atomicExch(status, 1);
+    if (threadIdx.x == 0 && status != nullptr) atomicOr(status, 1);
     for (int w = 0; w < 50; ++w) __nanosleep(20000);  // let copies in flight land before the smem goes away
     __syncthreads();
   }

@@ -1335,7 +1335,7 @@ tc_fwd_kernel(const __grid_constant__ TcMaps maps, const FwdParams p, const __gr
   tc_fence_before();
   __syncthreads();
   if (*abort_flag) {
-    if (threadIdx.x == 0 && status != nullptr) atomicExch(status, 1);
+    if (threadIdx.x == 0 && status != nullptr) atomicOr(status, 1);
     // give copies that are still in flight time to land before the smem goes away
     for (int w = 0; w < 50; ++w) __nanosleep(20000);
     __syncthreads();

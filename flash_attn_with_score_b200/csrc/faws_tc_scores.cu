@@ -214,7 +214,7 @@ tc_qk_scores_kernel(const __grid_constant__ ScMaps maps, const ScParams p, int* 
   tc_fence_before();
   __syncthreads();
   if (*abort_flag) {
-    if (threadIdx.x == 0 && status != nullptr) atomicExch(status, 1);
+    if (threadIdx.x == 0 && status != nullptr) atomicOr(status, 1);
     for (int w = 0; w < 50; ++w) __nanosleep(20000);  // let copies in flight land before the smem goes away
     __syncthreads();
   }
