@@ -36,7 +36,7 @@ EXPORTS = [
     "faws_window_backward_bytes",
     "faws_kv_cache_write", "faws_kv_cache_read", "faws_attention_with_kv_cache", "faws_kv_cache_workspace_bytes",
     "faws_total_attention", "faws_attention_backward", "faws_workspace_bytes", "faws_reduce_ranks", "faws_device_status",
-    "faws_selftest_wait_give_up", "faws_last_backend",
+    "faws_selftest_wait_give_up", "faws_selftest_kv_cache_give_up", "faws_last_backend",
     "faws_launch_count", "faws_strerror", "faws_version",
 ]
 
@@ -118,6 +118,7 @@ def load():
         "faws_kv_cache_read": (i32, cache + [C.POINTER(Tensor), C.POINTER(Tensor), i32, vp]),
         "faws_attention_with_kv_cache": (i32, [PP] + cache + [i32, i32, vp, sz, vp]),
         "faws_kv_cache_workspace_bytes": (sz, [PP]),
+        "faws_selftest_kv_cache_give_up": (i32, [PP] + cache + [i32, i32, i32, vp, sz, vp]),
         "faws_total_attention": (i32, [PP, vp, vp]),
         "faws_attention_backward": (i32, [PP, C.POINTER(Grads), vp, sz, vp]),
         "faws_workspace_bytes": (sz, [i32, PP, i32]),

@@ -887,8 +887,9 @@ size_t faws_kv_cache_workspace_bytes(const faws_problem* p) {
   return align256(cache_attn_workspace_bytes(p->D));
 }
 
-int faws_attention_with_kv_cache(const faws_problem* p, const faws_kv_cache* c, const faws_cache_batch* batch,
-                                 int32_t window, int32_t sinks, void* workspace, size_t workspace_bytes, void* stream) {
+static int cache_attention(const faws_problem* p, const faws_kv_cache* c, const faws_cache_batch* batch, int32_t window,
+                           int32_t sinks, int32_t tiles_at_most, long long wait_cycles, void* workspace, size_t workspace_bytes,
+                           void* stream) {
   if (p == nullptr || p->Hq <= 0 || p->Hk <= 0 || p->M <= 0 || p->Hq % p->Hk != 0) return FAWS_EINVAL;
   const int64_t rows = (int64_t)(p->Hq / p->Hk) * p->M;
   const int st = validate_cache(c, batch, rows);
@@ -910,6 +911,8 @@ int faws_attention_with_kv_cache(const faws_problem* p, const faws_kv_cache* c, 
   a.window = window == 0 || window > (1 << 30) ? 1 << 30 : window;
   a.sinks = sinks > (1 << 30) ? 1 << 30 : sinks;
   a.sm_scale = p->sm_scale;
+  a.tiles_at_most = tiles_at_most;
+  a.wait_cycles = wait_cycles;
   a.parts = static_cast<float*>(workspace);
   const cudaError_t e = launch_cache_attn(a, p->dtype, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) {
@@ -918,6 +921,17 @@ int faws_attention_with_kv_cache(const faws_problem* p, const faws_kv_cache* c, 
   }
   t_last_backend = FAWS_BACKEND_GENERIC;
   return FAWS_OK;
+}
+
+int faws_attention_with_kv_cache(const faws_problem* p, const faws_kv_cache* c, const faws_cache_batch* batch,
+                                 int32_t window, int32_t sinks, void* workspace, size_t workspace_bytes, void* stream) {
+  return cache_attention(p, c, batch, window, sinks, INT32_MAX, 4000000000ll, workspace, workspace_bytes, stream);
+}
+
+int faws_selftest_kv_cache_give_up(const faws_problem* p, const faws_kv_cache* c, const faws_cache_batch* batch,
+                                   int32_t window, int32_t sinks, int32_t tiles, void* workspace, size_t workspace_bytes,
+                                   void* stream) {
+  return cache_attention(p, c, batch, window, sinks, tiles, 2000000ll, workspace, workspace_bytes, stream);
 }
 
 int faws_reduce_ranks(const float* parts, int32_t n_ranks, int64_t count, float* out, void* stream) {

@@ -572,6 +572,8 @@ __global__ void __launch_bounds__(CTA_THREADS, CTAS_PER_SM) cache_attn_kernel(co
   __syncthreads();
   griddep_wait();
   griddep_launch_dependents();
+  // nothing to join, until this thread says so (a share whose waits give up may not come to that)
+  if (threadIdx.x == 0) part_header(p, blockIdx.x)->w = -1;
   if (warp == 0) {
     Walk first;
     Shares shares;
@@ -601,7 +603,6 @@ __global__ void __launch_bounds__(CTA_THREADS, CTAS_PER_SM) cache_attn_kernel(co
   __syncthreads();
   const bool any = bars->any != 0;
   Walk w = bars->walk;
-  if (!any && threadIdx.x == 0) part_header(p, blockIdx.x)->w = -1;
 
   if (any && warp == CONSUMERS) {
     // ------------------------------------------------------------ copies
@@ -648,7 +649,7 @@ __global__ void __launch_bounds__(CTA_THREADS, CTAS_PER_SM) cache_attn_kernel(co
         const Piece c = next;
         if (it + 1 < cnt) next = piece_of(it + 1);  // (its page comes while the tile before it waits for room)
         const int s = n % STAGES;
-        if (lane == 0) ok = mbar_wait(&bars->empty[s], ((n / STAGES) & 1) ^ 1, abort_flag);
+        if (lane == 0) ok = n < p.tiles_at_most && mbar_wait(&bars->empty[s], ((n / STAGES) & 1) ^ 1, abort_flag, p.wait_cycles);
         ok = __shfl_sync(0xffffffffu, ok, 0);
         if (!ok) break;
         unsigned char* dst = smem + s * L::kStage + off + (c.lo - c.t0) * bytes;
@@ -983,7 +984,8 @@ __global__ void __launch_bounds__(CTA_THREADS, CTAS_PER_SM) cache_attn_kernel(co
 
       for (int it = 0; ok && it < cnt; ++it, ++n) {
         const int t0 = w.span.tile(w.first + it) * TT, st = n % STAGES;
-        ok = mbar_wait(&bars->full[st], (n / STAGES) & 1, abort_flag);
+        // (of one mind: the lanes of a warp go on together, or none)
+        ok = __all_sync(0xffffffffu, mbar_wait(&bars->full[st], (n / STAGES) & 1, abort_flag, p.wait_cycles));
         if (!ok) break;
         const unsigned char* stage = smem + st * L::kStage;
         const int n0 = t0 + warp * 32;
@@ -1067,6 +1069,8 @@ __global__ void __launch_bounds__(256) cache_combine_kernel(const CacheAttnParam
   const int4 head = *part_header(p, c0);
   const int c1 = head.w;
   if (c1 <= c0) return;
+  // (no header of a call that ran to its end says anything else)
+  if (c1 >= (int)gridDim.x || (unsigned)head.x >= (unsigned)p.batch.B || (unsigned)head.y >= (unsigned)(p.cache.Hk * p.row_blocks)) return;
   const int hk = head.y / p.row_blocks, r0 = (head.y % p.row_blocks) * RT;
   for (int x = threadIdx.x; x < RT * (D / 4); x += 256) {
     const int row = x / (D / 4), d = (x % (D / 4)) * 4;
@@ -1126,8 +1130,9 @@ cudaError_t launch_attn_d(CacheAttnParams p, cudaStream_t s) {
   static PerDeviceOnce once;
   if (cudaError_t e = set_max_smem_once(once, cache_attn_kernel<T, D>, CacheSmem<D>::total); e != cudaSuccess) return e;
   p.row_blocks = (p.rows + RT - 1) / RT;
-  if (cudaError_t e = launch_overlapped(cache_attn_kernel<T, D>, dim3(p.grid), CTA_THREADS, CacheSmem<D>::total, s, p); e != cudaSuccess)
-    return e;
+  if (p.tiles_at_most >= 0)
+    if (cudaError_t e = launch_overlapped(cache_attn_kernel<T, D>, dim3(p.grid), CTA_THREADS, CacheSmem<D>::total, s, p); e != cudaSuccess)
+      return e;
   return launch_overlapped(cache_combine_kernel<T, D>, dim3(p.grid), 256, 0, s, p);
 }
 template <typename T>

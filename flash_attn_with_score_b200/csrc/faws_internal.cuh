@@ -230,6 +230,10 @@ struct CacheAttnParams {
   int G, M, rows;     // rows: G * M, of a kv head
   int window, sinks;  // at most 2^30
   float sm_scale;
+  // Self-test of the give-up path: a CTA's copies end after so many tiles, its waits after so many cycles; below 0, only the joining
+  // kernel runs.
+  int tiles_at_most;
+  long long wait_cycles;
   // set by the launcher
   int row_blocks, grid, min_tiles, vec_out;
   float* parts;       // workspace

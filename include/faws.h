@@ -401,6 +401,16 @@ int faws_device_status(int32_t reset);
  */
 int faws_selftest_wait_give_up(void* stream);
 
+/*
+ * The same of faws_attention_with_kv_cache, whose arguments it takes: the copies of each CTA end after `tiles` tiles of 128
+ * tokens, and what waits for more gives up after about a millisecond.  CTAs with more to do raise the status word and
+ * return; out and log_normalizer are invalid, nothing else is touched.  tiles < 0: only the kernel that joins the CTAs'
+ * parts runs, on what the workspace holds; entries that no call leaves there are passed over.
+ */
+int faws_selftest_kv_cache_give_up(const faws_problem* p, const faws_kv_cache* c, const faws_cache_batch* batch,
+                                   int32_t window, int32_t sinks, int32_t tiles, void* workspace, size_t workspace_bytes,
+                                   void* stream);
+
 /* Which kernel family the calling thread's last successful call used
  * (FAWS_BACKEND_GENERIC or FAWS_BACKEND_TCGEN05; 0 before any call) and how
  * many kernels this library has launched from this process. */
