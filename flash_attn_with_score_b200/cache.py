@@ -4,7 +4,7 @@ The operators take sequences as the rest of the package does: tensors (B, H, row
 sequence.  ``lengths[b]`` counts the tokens of sequence b, those of the call among them, so row m of M stands for position
 ``lengths[b] - M + m``; rows before position 0 are padding.  ``page_table[b, n // page_size]`` is the page that holds position n.
 Both are int32 tensors on the cache's device, so that a decoding step can be captured in a graph and replayed with
-others in place.
+others in place (between calls, in stream order: while one runs they stay as they are).
 
 Positions, pages and lengths are known to the device alone.  What does not exist there is never touched: rows on a page outside
 the cache, or at a position behind the table's last page, are not written and read as NaN, as do outputs that see such keys (a

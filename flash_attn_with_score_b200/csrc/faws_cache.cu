@@ -468,7 +468,8 @@ __device__ __forceinline__ bool walk_begin(const CacheAttnParams& p, int lane, W
   w->end = sh.begin(min((int)blockIdx.x + 1, sh.shares));
   if (w->at >= w->end) return false;
   int base = 0;
-  for (int b0 = 0;; b0 += 32) {
+  // (lengths that change under the call, which they must not, end the walk here or in walk_next, not the batch)
+  for (int b0 = 0; b0 < p.batch.B; b0 += 32) {
     const int all = p.batch.B <= 32 ? total : chunk(b0);  // (one chunk: as it was)
     const unsigned past = __ballot_sync(0xffffffffu, base + n > w->at);
     if (past != 0u) {
@@ -477,15 +478,15 @@ __device__ __forceinline__ bool walk_begin(const CacheAttnParams& p, int lane, W
       w->b = b0 + first;
       w->span = span_of(p, w->b, &bad);
       const int off = w->at - base - (first == 0 ? 0 : before);
-      w->item = off / w->span.nt;
+      w->item = off / max(w->span.nt, 1);
       w->first = off - w->item * w->span.nt;
-      break;
+      return w->span.nt > 0 && w->item < items;
     }
     base += all;
   }
-  return true;
+  return false;
 }
-__device__ __forceinline__ bool walk_next(const CacheAttnParams& p, Walk* w) {
+__device__ __forceinline__ bool walk_next(const CacheAttnParams& p, Walk* w, volatile int* abort_flag) {
   w->at += w->count();
   if (w->at >= w->end) return false;
   w->first = 0;
@@ -493,9 +494,12 @@ __device__ __forceinline__ bool walk_next(const CacheAttnParams& p, Walk* w) {
     w->item = 0;
     bool bad = false;
     do {
-      ++w->b;
+      if (++w->b >= p.batch.B) {  // (the list has more tiles, so a later sequence has some)
+        *abort_flag = 1;
+        return false;
+      }
       w->span = span_of(p, w->b, &bad);
-    } while (w->span.nt == 0);  // (the list has more tiles, so a later sequence has some)
+    } while (w->span.nt == 0);
   }
   return true;
 }
@@ -669,7 +673,7 @@ __global__ void __launch_bounds__(CTA_THREADS, CTAS_PER_SM) cache_attn_kernel(co
           mbar_arrive(&bars->full[s]);
         }
       }
-    } while (ok && walk_next(p, &w));
+    } while (ok && walk_next(p, &w, abort_flag));
     if (bad && p.status != nullptr) atomicOr(p.status, kBadPage);
   } else if (any) {
     // ------------------------------------------------------------ rows
@@ -1048,8 +1052,8 @@ __global__ void __launch_bounds__(CTA_THREADS, CTAS_PER_SM) cache_attn_kernel(co
         const int end = begins && !ends ? bars->shares.of(w.at + w.span.nt - 1) : -1;
         *part_header(p, blockIdx.x) = make_int4(w.b, w.item, 0, end);
       }
-      ok = !consumers_any(!ok);  // (all of them go on, or none)
-    } while (ok && walk_next(p, &w));
+      ok = ok && walk_next(p, &w, abort_flag);
+    } while (!consumers_any(!ok));  // (all of them go on, or none)
   }
   __syncthreads();
   if (*abort_flag) {

@@ -341,7 +341,7 @@ typedef struct faws_kv_cache {
  * counts the tokens of sequence b, those of the call among them: the calls below take `rows` (M) rows per sequence, row m
  * being position lengths[b] - rows + m (aligned to the end, as causal masks are).  Rows before position 0 are padding.  A head
  * has at most 2^30 rows of a sequence (of attention: a kv head, over the query heads that share it).
- * Both arrays are on the device.  A length below 0 is taken as 0.  Positions from max_pages * page_size on (2^30 - 1 at most)
+ * Both arrays are on the device and stay as they are until the call has run.  A length below 0 is taken as 0.  Positions from max_pages * page_size on (2^30 - 1 at most)
  * do not exist, nor do those on a page outside [0, pages): they are not touched.  A length below 0 or with such positions and a
  * page out of range raise the device's status word (faws_device_status: 2).
  */
