@@ -188,6 +188,13 @@ PyObject* window(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// Runs a call that launches, without Python's lock: it waits where the launch queue is full.
+template <typename Call>
+int unlocked(Call call) {
+  pybind11::gil_scoped_release no_gil;
+  return call();
+}
+
 // The page table and lengths of a cache's call as the kernels take them, for B sequences on `dev`.
 bool plain_batch(PyObject* table, PyObject* lengths, int64_t B, c10::Device dev, faws_cache_batch* out) {
   if (!usual_cuda(table) || !usual_cuda(lengths)) return false;
@@ -228,7 +235,9 @@ PyObject* cache_write(PyObject*, PyObject* const* a, Py_ssize_t n) {
   faws_cache_batch b;
   if (!plain_batch(a[4], a[5], k.size(0), dev, &b)) Py_RETURN_NONE;
   const faws_tensor kt = view(k), vt = view(v);
-  check(faws_kv_cache_write(c, &b, &kt, &vt, (int32_t)k.size(2), current_stream(k)), "faws_kv_cache_write");
+  void* stream = current_stream(k);
+  const int32_t rows = (int32_t)k.size(2);
+  check(unlocked([&] { return faws_kv_cache_write(c, &b, &kt, &vt, rows, stream); }), "faws_kv_cache_write");
   Py_RETURN_TRUE;
   END_HANDLE_TH_ERRORS
 }
@@ -252,7 +261,8 @@ PyObject* cache_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const auto options = l.options().dtype(cache_type(c)).requires_grad(false);
   at::Tensor k = at::empty({l.size(0), c->Hk, rows, c->D}, options), v = at::empty({l.size(0), c->Hk, rows, c->D}, options);
   const faws_tensor kt = view(k), vt = view(v);
-  check(faws_kv_cache_read(c, &b, &kt, &vt, (int32_t)rows, current_stream(k)), "faws_kv_cache_read");
+  void* stream = current_stream(k);
+  check(unlocked([&] { return faws_kv_cache_read(c, &b, &kt, &vt, (int32_t)rows, stream); }), "faws_kv_cache_read");
   return wrap(std::move(k), std::move(v));
   END_HANDLE_TH_ERRORS
 }
@@ -290,7 +300,8 @@ PyObject* cache_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   }
   const size_t bytes = faws_kv_cache_workspace_bytes(&p);
   const at::Tensor ws = bytes_like(q, bytes);
-  check(faws_attention_with_kv_cache(&p, c, &b, (int32_t)window, (int32_t)sinks, ws.data_ptr(), bytes, current_stream(q)),
+  void *scratch = ws.data_ptr(), *stream = current_stream(q);
+  check(unlocked([&] { return faws_attention_with_kv_cache(&p, c, &b, (int32_t)window, (int32_t)sinks, scratch, bytes, stream); }),
         "faws_attention_with_kv_cache");
   return wrap(std::move(out), std::move(L));
   END_HANDLE_TH_ERRORS
