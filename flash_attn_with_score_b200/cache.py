@@ -81,7 +81,8 @@ def _run(cache, name, *args):
 
 def kv_cache_write(cache, k, v, page_table, lengths):
     """Quantises k and v (B, Hk, M, D), the last M rows of each sequence, into the cache; padding rows are skipped.  Rows of one
-    call are to go to different places (a page that several sequences share may be read by all, written by none)."""
+    call are to go to different places (a page that several sequences share may be read by all, written by none).  No gradients: k and v
+    that want one are refused."""
     if type(cache) is KVCache4 and _lib.plain("cache_write", *cache._plain, k, v, page_table, lengths):
         return
     assert k.dim() == 4 and k.shape == v.shape, "k and v must have the same (B, Hk, M, D)"
@@ -91,6 +92,8 @@ def kv_cache_write(cache, k, v, page_table, lengths):
     if k.dtype != cache.dtype or v.dtype != cache.dtype:
         raise TypeError(f"k and v must be {cache.dtype} as the cache is, got {k.dtype}, {v.dtype}")
     assert k.device == cache.device and v.device == cache.device, "k and v must be on the cache's device"
+    if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad):
+        raise RuntimeError("kv_cache_write has no backward pass: call it under torch.no_grad(), or with detached k and v")
     if B == 0 or M == 0:
         return
     k, v = maybe_contiguous(k), maybe_contiguous(v)

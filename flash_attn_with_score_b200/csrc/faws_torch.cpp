@@ -230,6 +230,7 @@ PyObject* cache_write(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (c == nullptr) return nullptr;
   if (!plain(a[2]) || !plain(a[3]) || modes_on() || dev.index() != c10::cuda::current_device()) Py_RETURN_NONE;
   const at::Tensor &k = THPVariable_Unpack(a[2]), &v = THPVariable_Unpack(a[3]);
+  if ((k.requires_grad() || v.requires_grad()) && at::GradMode::is_enabled()) Py_RETURN_NONE;
   if (k.sizes() != v.sizes() || k.size(1) != c->Hk || k.size(3) != c->D || k.size(2) > INT32_MAX) Py_RETURN_NONE;
   if (k.scalar_type() != cache_type(c) || v.scalar_type() != cache_type(c) || k.device() != dev || v.device() != dev) Py_RETURN_NONE;
   faws_cache_batch b;
