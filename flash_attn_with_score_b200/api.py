@@ -25,6 +25,7 @@ import math
 import struct
 
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 from . import _lib
 
@@ -239,6 +240,12 @@ def attention(q, k, v, causal=False, sm_scale=None, dropout_p=0.0,
 _NO_LIMIT = 2 ** 31 - 1
 
 
+def _no_tangents(name, *tensors):
+    """Refuses tensors with a forward-mode tangent, which the result would lack."""
+    if getattr(forward_ad, "_current_level", 0) >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError(f"{name} has no forward-mode derivative")
+
+
 def _window_forward(q, k, v, window, sinks, sm_scale, need_L, backend, kv_splits):
     c = _Call(q, k, v, True, sm_scale, 0.0, need_L=need_L, backend=backend)
     n_splits = int(c.lib.faws_window_split_plan(C.byref(c.p), window, sinks)) if kv_splits is None else int(kv_splits)
@@ -287,6 +294,7 @@ def attention_with_window(q, k, v, window, sinks=0, sm_scale=None, return_log_no
     window, sinks = min(int(window), _NO_LIMIT), min(int(sinks), _NO_LIMIT)
     assert window >= 1, "window must be at least 1"
     assert sinks >= 0, "sinks must not be negative"
+    _no_tangents("attention_with_window", q, k, v)
     if backend is None and kv_splits is None:
         got = _lib.plain("window", q, k, v, window, sinks, sm_scale, return_log_normalizer)
         if got is not None:

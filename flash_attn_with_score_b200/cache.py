@@ -18,7 +18,7 @@ import math
 import torch
 
 from . import _lib
-from .api import _DTYPES, _NO_LIMIT, _raw_stream, _tensor, maybe_contiguous
+from .api import _DTYPES, _NO_LIMIT, _no_tangents, _raw_stream, _tensor, maybe_contiguous
 
 
 class KVCache4:
@@ -83,6 +83,7 @@ def kv_cache_write(cache, k, v, page_table, lengths):
     """Quantises k and v (B, Hk, M, D), the last M rows of each sequence, into the cache; padding rows are skipped.  Rows of one
     call are to go to different places (a page that several sequences share may be read by all, written by none).  No gradients: k and v
     that want one are refused."""
+    _no_tangents("kv_cache_write", k, v)
     if type(cache) is KVCache4 and _lib.plain("cache_write", *cache._plain, k, v, page_table, lengths):
         return
     assert k.dim() == 4 and k.shape == v.shape, "k and v must have the same (B, Hk, M, D)"
@@ -127,6 +128,7 @@ def attention_with_kv_cache(q, cache, page_table, lengths, window=None, sinks=0,
     assert window is None or window >= 1, "window must be at least 1"
     assert sinks >= 0, "sinks must not be negative"
     window, sinks = min(int(window), _NO_LIMIT) if window is not None else 0, min(int(sinks), _NO_LIMIT)
+    _no_tangents("attention_with_kv_cache", q)
     if type(cache) is KVCache4:
         got = _lib.plain("cache_attention", *cache._plain, q, page_table, lengths, window, sinks, sm_scale, return_log_normalizer)
         if got is not None:
