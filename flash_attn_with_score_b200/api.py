@@ -83,9 +83,10 @@ class _Call:
             raise TypeError(f"q, k, v must share dtype float16 or bfloat16, got {q.dtype}, {k.dtype}, {v.dtype}")
         if sm_scale is None:
             sm_scale = 1.0 / math.sqrt(D)
+        self.dev = q.device
+        assert all(t is None or t.device == self.dev for t in (k, v, out, L)), "the tensors of a call must be on one device"
         self.q, self.k, self.v = maybe_contiguous(q), maybe_contiguous(k), maybe_contiguous(v)
         self.B, self.H, self.Hk, self.M, self.N, self.D = B, H, Hk, M, N, D
-        self.dev = q.device
         self.lib = _lib.load()
         if out is None:
             out = torch.empty_like(self.q)
@@ -326,6 +327,7 @@ def attention_with_scores(q, k, v, causal=False, sm_scale=None, dropout_p=0.0,
         scores = torch.empty((c.B, c.H, c.M, c.N), device=c.dev, dtype=scores_dtype)
     else:
         assert scores.shape == (c.B, c.H, c.M, c.N) and scores.dtype == scores_dtype and scores.is_contiguous()
+        assert scores.device == c.dev, "the tensors of a call must be on one device"
     sd = _lib.SCORES_F32 if scores_dtype == torch.float32 else _lib.SCORES_INPUT
     c.run("faws_attention_with_scores", C.c_void_p(scores.data_ptr()), sd, _f32_bits(masked_value))
     return c.out, scores
