@@ -274,7 +274,11 @@ class _WindowFunction(torch.autograd.Function):
         q, k, v, o, L = ctx.saved_tensors
         if do is None:
             return (*map(torch.zeros_like, (q, k, v)), *(None,) * 5)
-        do = maybe_contiguous(do)
+        # (a saved-tensor hook may have brought back other tensors than were saved)
+        if not (o.shape == q.shape == do.shape and L.shape == q.shape[:3] and k.shape == v.shape and L.dtype == torch.float32
+                and q.dtype == k.dtype == v.dtype == o.dtype == do.dtype and q.is_cuda and do.device == q.device):
+            raise RuntimeError("attention_with_window: a saved tensor came back with another shape, type or device")
+        do, o, L = maybe_contiguous(do), maybe_contiguous(o), L.contiguous()
         c = _Call(q, k, v, True, ctx.sm_scale, 0.0, out=o, L=L, backend=ctx.backend)
         dq, dk, dv = torch.empty_like(c.q), torch.empty_like(c.k), torch.empty_like(c.v)
         g = _lib.Grads(_tensor(do), _tensor(dq), _tensor(dk), _tensor(dv))

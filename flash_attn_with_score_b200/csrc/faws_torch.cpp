@@ -117,13 +117,24 @@ struct WindowFunction : public torch::autograd::Function<WindowFunction> {
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
     TORCH_CHECK(!at::GradMode::is_enabled(), "attention_with_window has no second derivative (create_graph)");
-    const auto saved = ctx->get_saved_variables();
+    auto saved = ctx->get_saved_variables();
+    // (a saved-tensor hook may have brought back other tensors than were saved: strides are those of now)
+    for (int i = 0; i < 4; ++i)
+      if (saved[i].dim() == 4 && saved[i].stride(3) != 1) saved[i] = saved[i].contiguous();
     const at::Tensor &q = saved[0], &k = saved[1], &v = saved[2], &out = saved[3], &L = saved[4];
     const at::Tensor none;
+    if (grads[0].defined()) {
+      const at::Tensor& g = grads[0];
+      auto like = [&](const at::Tensor& t) { return t.dim() == 4 && t.scalar_type() == g.scalar_type() && t.device() == g.device(); };
+      const bool same = like(q) && like(k) && like(v) && like(out) && q.sizes() == g.sizes() && out.sizes() == g.sizes() &&
+                        v.sizes() == k.sizes() && k.size(0) == q.size(0) && k.size(3) == q.size(3) && k.size(1) > 0 &&
+                        q.size(1) % k.size(1) == 0 && L.sizes() == q.sizes().slice(0, 3) && L.scalar_type() == at::kFloat &&
+                        L.device() == g.device();
+      TORCH_CHECK(same, "attention_with_window: a saved tensor came back with another shape, type or device");
+    }
     if (!grads[0].defined()) return {at::zeros_like(q), at::zeros_like(k), at::zeros_like(v), none, none, none};
     const at::Tensor dout = grads[0].stride(3) == 1 ? grads[0] : grads[0].contiguous();
     at::Tensor dq = at::empty_like(q), dk = at::empty_like(k), dv = at::empty_like(v);
-    // (a saved-tensor hook may have brought back other tensors than were saved: strides are those of now)
     faws_problem p{};
     p.B = (int32_t)q.size(0); p.Hq = (int32_t)q.size(1); p.Hk = (int32_t)k.size(1);
     p.M = p.m_end = (int32_t)q.size(2); p.N = (int32_t)k.size(2); p.D = (int32_t)q.size(3);
