@@ -55,12 +55,13 @@ class KVCache4:
         super().__setattr__(name, value)
 
 
-def _batch(cache, page_table, lengths, B):
+def _batch(cache, page_table, lengths, B, rows):
     if not isinstance(cache, KVCache4):
         raise TypeError("cache must be a KVCache4")
     assert page_table.dim() == 2 and page_table.shape[0] == B and page_table.shape[1] > 0, (
         f"page_table must be ({B}, pages of a sequence), got {tuple(page_table.shape)}")
     assert lengths.shape == (B,), f"lengths must be ({B},), got {tuple(lengths.shape)}"
+    assert max(B, rows, page_table.shape[1]) < 2 ** 31, "sequences, rows and pages of a sequence are counted in 32 bits"
     if page_table.dtype != torch.int32 or lengths.dtype != torch.int32:
         raise TypeError("page_table and lengths must be int32")
     assert page_table.device == cache.device and lengths.device == cache.device, "page_table and lengths must be on the cache's device"
@@ -88,7 +89,7 @@ def kv_cache_write(cache, k, v, page_table, lengths):
         return
     assert k.dim() == 4 and k.shape == v.shape, "k and v must have the same (B, Hk, M, D)"
     B, Hk, M, D = k.shape
-    table, lens, batch = _batch(cache, page_table, lengths, B)
+    table, lens, batch = _batch(cache, page_table, lengths, B, M)
     assert Hk == cache.heads and D == cache.head_dim, f"rows are ({Hk}, {D}) heads and dims, the cache has ({cache.heads}, {cache.head_dim})"
     if k.dtype != cache.dtype or v.dtype != cache.dtype:
         raise TypeError(f"k and v must be {cache.dtype} as the cache is, got {k.dtype}, {v.dtype}")
@@ -109,7 +110,7 @@ def kv_cache_read(cache, page_table, lengths, rows):
         if got is not None:
             return got
     B = lengths.shape[0]
-    table, lens, batch = _batch(cache, page_table, lengths, B)
+    table, lens, batch = _batch(cache, page_table, lengths, B, rows)
     assert rows >= 0, "rows must not be negative"
     shape = (B, cache.heads, rows, cache.head_dim)
     k, v = (torch.empty(shape, dtype=cache.dtype, device=cache.device) for _ in range(2))
@@ -135,7 +136,7 @@ def attention_with_kv_cache(q, cache, page_table, lengths, window=None, sinks=0,
             return got
     assert q.dim() == 4, "q must be (B, Hq, M, D)"
     B, H, M, D = q.shape
-    table, lens, batch = _batch(cache, page_table, lengths, B)
+    table, lens, batch = _batch(cache, page_table, lengths, B, max(H, M))
     assert D == cache.head_dim, f"feature size of q is {D}, the cache's {cache.head_dim}"
     assert H > 0 and H % cache.heads == 0, "number of heads in q must be a multiple of that in the cache"
     if q.dtype != cache.dtype:

@@ -502,8 +502,9 @@ int validate_cache(const faws_kv_cache* c, const faws_cache_batch* b, int64_t ro
   if (b->page_table == nullptr || b->lengths == nullptr || b->table_stride < 0) return FAWS_EINVAL;
   for (const void* x : {c->k_codes, c->v_codes, c->k_scales, c->v_scales})
     if (x == nullptr || reinterpret_cast<uintptr_t>(x) % 16 != 0) return FAWS_EINVAL;
-  // rows are counted in 32 bits together with positions; a block has 2048 elements of these rows, a grid 2^31 - 1 blocks
-  if (rows > (1 << 30) || (int64_t)b->B * c->Hk > (int64_t(1) << 40) / (rows * c->D)) return FAWS_EINVAL;
+  // rows are counted in 32 bits together with positions; a sequence and head has a block of its own, or one for at least 2048
+  // elements of its rows, a grid 2^31 - 1 blocks
+  if (rows > (1 << 30) || (int64_t)b->B * c->Hk > INT32_MAX / ((rows * c->D + 2047) / 2048)) return FAWS_EINVAL;
   return FAWS_OK;
 }
 CacheParams make_cache(const faws_kv_cache* c) {
