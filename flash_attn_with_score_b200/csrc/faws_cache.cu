@@ -19,7 +19,6 @@
 // half, and after a rotation by 8 the next two do: the mantissa of a half-precision number.
 #include <cuda.h>
 
-#include <algorithm>
 #include <type_traits>
 
 #include "faws_internal.cuh"
@@ -306,8 +305,8 @@ __device__ __forceinline__ void read_rows(const CacheParams& c, const CacheRows&
 }
 
 // Keys in the first half of the grid, values in the second.  CTAs whose rows all exist, on one page, with 16-byte accesses, go
-// without the checks for each row (bf16 and fp16, 4 sequences of 8192 rows of 8 heads of 128: written in 42.7 us and read in 43.7 and
-// 50.8 with them).
+// without the checks for each row (4 sequences of 8192 rows of 8 heads of 128, inputs not in L2: bf16 and fp16 written in 38.9 us, read
+// in 35.6 and 38.9; with the checks 45.1, 52.0 and 55.3).
 template <typename T, int D, bool WRITE, int EACH>
 __global__ void __launch_bounds__(256) cache_rows_kernel(const CacheParams c, const CacheBatch bt, const CacheRows r, int* status) {
   griddep_wait();
@@ -344,7 +343,7 @@ __global__ void __launch_bounds__(256) cache_rows_kernel(const CacheParams c, co
 // adds up the parts of each item in order.
 //   warp 4      brings tiles into shared memory: codes and scales of a page and head are one bulk copy each
 //   warps 0-3   take 32 tokens of a tile each, with a running maximum, sum and output of their own, merged at the end
-// Matrix instructions are mma.sync m16n8k16 in fp16: a tile has 8 or 16 rows, and the operands come out of registers, where
+// Matrix instructions are mma.sync m16n8k16 in fp16: a tile has 8 rows, and the operands come out of registers, where
 // a nibble n in bits 2..5 of a half IS the number n 2^-22 (a subnormal): unpacking is one AND per pair, one rotation
 // per two.  Nibbles in bits 6..9 are 16 n 2^-22: the query's elements there (the output's rows there) carry 1/16.  The
 // matrix instructions align a subnormal as they do 2^-14, so that its products keep 2^-16 of a code, for nibbles in bits 6..9
@@ -356,8 +355,9 @@ __global__ void __launch_bounds__(256) cache_rows_kernel(const CacheParams c, co
 //                                                  with the same rounded weights, 16 tokens at a time: summed apart, the two would
 //                                                  grow with the tokens and lose in their difference what long contexts average out
 //                                                  (64 x 16384 tokens, fp16: 3.3e-4 of the output against 2.9e-4).
-// Weights are fp16: 2^-12 of each.  The running maximum is that of S + log2 s, so that P s stays within fp16 for values of
-// any size; what falls below 2^-24 of the largest weighted value is lost.
+// Weights are fp16: 2^-11 of each.  The running maximum is that of S + log2 s, s the largest scale of the token's value, so that
+// P s stays within fp16 for values of any size.  Below 2^-14 of the largest P s weights are subnormal and off by up to 2^-25 of it:
+// one maximum for all groups of 32 channels, so a group of values a power of two below its neighbours has as many bits less there.
 constexpr int RT = 8;         // rows of a row block: the width of a matrix instruction
 constexpr int TT = 128;       // tokens of a tile
 constexpr int STAGES = 3;
@@ -427,7 +427,7 @@ struct Shares {
   int shares, per, more;  // the first `more` shares have one tile more
   Shares() = default;
   __device__ __forceinline__ Shares(const CacheAttnParams& p, int total) {
-    shares = max(1, min(p.grid, (total + p.min_tiles - 1) / p.min_tiles));
+    shares = max(1, min(p.grid, total));
     per = total / shares;
     more = total - per * shares;
   }
@@ -560,7 +560,6 @@ __global__ void __launch_bounds__(CTA_THREADS, CTAS_PER_SM) cache_attn_kernel(co
   using L = CacheSmem<D>;
   constexpr int NG = L::NG;
   constexpr int MT = D >= 32 ? 2 : 1;  // 16-row tiles of a group's output
-  constexpr int NB = RT / 8;           // blocks of 8 rows
   extern __shared__ __align__(128) unsigned char smem[];
   CacheBars* bars = reinterpret_cast<CacheBars*>(smem + L::bar_off);
   volatile int* abort_flag = &bars->abort_flag;
@@ -697,13 +696,12 @@ __global__ void __launch_bounds__(CTA_THREADS, CTAS_PER_SM) cache_attn_kernel(co
       const int hk = w.item / p.row_blocks, r0 = (w.item % p.row_blocks) * RT, cnt = w.count();
       const int end = w.span.len + tokens_beyond(p, w.b);  // one behind the last row's position
       // ---- the rows' queries as fp16 operands, and -8 sum of each group; a lane loads row g of 8
-      uint32_t q[NB][NG][2][2];
-      uint64_t qbias[NB][NG];    // of rows 2 t and 2 t + 1, as f
-      float f[NB][2];
-      int hi_row[NB][2];         // a row sees keys [hi_row - window, hi_row) and the sinks before hi_row
-#pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
-        const int r = r0 + nb * 8 + g;
+      uint32_t q[NG][2][2];
+      uint64_t qbias[NG];    // of rows 2 t and 2 t + 1, as f
+      float f[2];
+      int hi_row[2];         // a row sees keys [hi_row - window, hi_row) and the sinks before hi_row
+      {
+        const int r = r0 + g;
         const bool real = r < p.rows;
         const int head = r / p.M, i = r - head * p.M;
         float x[NG][8];
@@ -729,8 +727,8 @@ __global__ void __launch_bounds__(CTA_THREADS, CTAS_PER_SM) cache_attn_kernel(co
         // rows 2 t and 2 t + 1 are loaded by the lanes 8 t and 8 t + 4
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          f[nb][c] = __shfl_sync(0xffffffffu, my_f, 8 * t + 4 * c);
-          hi_row[nb][c] = __shfl_sync(0xffffffffu, my_hi, 8 * t + 4 * c);
+          f[c] = __shfl_sync(0xffffffffu, my_f, 8 * t + 4 * c);
+          hi_row[c] = __shfl_sync(0xffffffffu, my_hi, 8 * t + 4 * c);
         }
 #pragma unroll
         for (int gi = 0; gi < NG; ++gi) {
@@ -744,29 +742,26 @@ __global__ void __launch_bounds__(CTA_THREADS, CTAS_PER_SM) cache_attn_kernel(co
           sum += __shfl_xor_sync(0xffffffffu, sum, 1);
           sum += __shfl_xor_sync(0xffffffffu, sum, 2);
           sum *= -8.f * 2.384185791015625e-7f;
-          qbias[nb][gi] = pack_f32x2(__shfl_sync(0xffffffffu, sum, 8 * t), __shfl_sync(0xffffffffu, sum, 8 * t + 4));
+          qbias[gi] = pack_f32x2(__shfl_sync(0xffffffffu, sum, 8 * t), __shfl_sync(0xffffffffu, sum, 8 * t + 4));
           auto pair = [&](int a, int b) {
             return (uint32_t)__half_as_ushort(h[a]) | (uint32_t)__half_as_ushort(h[b]) << 16;
           };
           // element y of a word is nibble y: registers (0, 4), (1, 5), (2, 6), (3, 7)
-          q[nb][gi][0][0] = pair(0, 4);
-          q[nb][gi][0][1] = pair(1, 5);
-          q[nb][gi][1][0] = pair(2, 6);
-          q[nb][gi][1][1] = pair(3, 7);
+          q[gi][0][0] = pair(0, 4);
+          q[gi][0][1] = pair(1, 5);
+          q[gi][1][0] = pair(2, 6);
+          q[gi][1][1] = pair(3, 7);
         }
       }
-      float o[NB][NG][MT][4], m[NB][2], l[NB][2];
+      float o[NG][MT][4], m[2], l[2];
+      m[0] = m[1] = FAWS_NEG_INF;
+      l[0] = l[1] = 0.f;
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
-        m[nb][0] = m[nb][1] = FAWS_NEG_INF;
-        l[nb][0] = l[nb][1] = 0.f;
+      for (int gi = 0; gi < NG; ++gi)
 #pragma unroll
-        for (int gi = 0; gi < NG; ++gi)
+        for (int c = 0; c < 4; ++c)
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt) o[nb][gi][mt][c] = 0.f;
-      }
+          for (int mt = 0; mt < MT; ++mt) o[gi][mt][c] = 0.f;
       // of the first, the last row (rows whose own key is behind `len` become NaN, whatever they take part in)
       const int hi_first = end - p.M + 1, lo_last = end - p.window;
 
@@ -818,8 +813,8 @@ __global__ void __launch_bounds__(CTA_THREADS, CTAS_PER_SM) cache_attn_kernel(co
             }
           } else sc[0] = reinterpret_cast<const uint64_t*>(table)[kv * 32 + at];
         };
-        // scores without the rows' factors f: [part][rows nb * 8 + 2 t, + 1][token g, g + 8]
-        uint64_t s[2][NB][2];
+        // scores without the rows' factors f: [part][rows 2 t, 2 t + 1][token g, g + 8]
+        uint64_t s[2][2];
 #pragma unroll
         for (int part = 0; part < 2; ++part) {
           uint32_t kw[2][NG];
@@ -839,95 +834,83 @@ __global__ void __launch_bounds__(CTA_THREADS, CTAS_PER_SM) cache_attn_kernel(co
             const uint32_t y0 = __funnelshift_r(kw[0][gi], kw[0][gi], 8), y1 = __funnelshift_r(kw[1][gi], kw[1][gi], 8);
             const uint32_t a0[4] = {kw[0][gi] & kLow, kw[1][gi] & kLow, kw[0][gi] & kHigh, kw[1][gi] & kHigh};
             const uint32_t a1[4] = {y0 & kLow, y1 & kLow, y0 & kHigh, y1 & kHigh};
+            float acc[4];
+            mma_f16_first(acc, a0, q[gi][0][0], q[gi][0][1]);
+            mma_f16(acc, a1, q[gi][1][0], q[gi][1][1]);
 #pragma unroll
-            for (int nb = 0; nb < NB; ++nb) {
-              float acc[4];
-              mma_f16_first(acc, a0, q[nb][gi][0][0], q[nb][gi][0][1]);
-              mma_f16(acc, a1, q[nb][gi][1][0], q[nb][gi][1][1]);
-#pragma unroll
-              for (int half = 0; half < 2; ++half) {
-                const uint64_t x = add_f32x2(pack_f32x2(acc[2 * half], acc[2 * half + 1]), qbias[nb][gi]);
-                s[part][nb][half] = gi == 0 ? mul_f32x2(x, sc[half][gi]) : fma_f32x2(x, sc[half][gi], s[part][nb][half]);
-              }
+            for (int half = 0; half < 2; ++half) {
+              const uint64_t x = add_f32x2(pack_f32x2(acc[2 * half], acc[2 * half + 1]), qbias[gi]);
+              s[part][half] = gi == 0 ? mul_f32x2(x, sc[half][gi]) : fma_f32x2(x, sc[half][gi], s[part][half]);
             }
           }
         }
         // ---- running maximum, moved only when a weighted value would exceed 2^8
-        [[maybe_unused]] uint32_t hidden[NB];  // bit 4 part + 2 half + row
-        float top[NB][2], ev[2][2];
+        [[maybe_unused]] uint32_t hidden;  // bit 4 part + 2 half + row
+        float top[2], ev[2][2];
         bool need = false;
 #pragma unroll
         for (int part = 0; part < 2; ++part)
 #pragma unroll
           for (int half = 0; half < 2; ++half) ev[part][half] = __shfl_sync(0xffffffffu, my_ev, part * 16 + half * 8 + krow);
+        hidden = 0u;
+        float x[2][2][2];
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb) {
-          hidden[nb] = 0u;
-          float x[2][2][2];
+        for (int part = 0; part < 2; ++part)
 #pragma unroll
-          for (int part = 0; part < 2; ++part)
+          for (int half = 0; half < 2; ++half) {
+            float y[2];
+            unpack_f32x2(s[part][half], y[0], y[1]);
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              float y[2];
-              unpack_f32x2(s[part][nb][half], y[0], y[1]);
-#pragma unroll
-              for (int c = 0; c < 2; ++c) {
-                x[c][part][half] = fmaf(y[c], f[nb][c], ev[part][half]);
-                if constexpr (kMasked) {
-                  const int j = n0 + part * 16 + half * 8 + krow;
-                  if (!(j < hi_row[nb][c] && (j >= hi_row[nb][c] - p.window || j < p.sinks))) {
-                    x[c][part][half] = FAWS_NEG_INF;
-                    hidden[nb] |= 1u << (part * 4 + half * 2 + c);
-                  }
+            for (int c = 0; c < 2; ++c) {
+              x[c][part][half] = fmaf(y[c], f[c], ev[part][half]);
+              if constexpr (kMasked) {
+                const int j = n0 + part * 16 + half * 8 + krow;
+                if (!(j < hi_row[c] && (j >= hi_row[c] - p.window || j < p.sinks))) {
+                  x[c][part][half] = FAWS_NEG_INF;
+                  hidden |= 1u << (part * 4 + half * 2 + c);
                 }
               }
             }
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            top[nb][c] = fmax3(fmaxf(x[c][0][0], x[c][0][1]), x[c][1][0], x[c][1][1]);
-            need = need || top[nb][c] > m[nb][c] + 8.f;
           }
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          top[c] = fmax3(fmaxf(x[c][0][0], x[c][0][1]), x[c][1][0], x[c][1][1]);
+          need = need || top[c] > m[c] + 8.f;
         }
         if (__any_sync(0xffffffffu, need)) {
+          float alpha[2];
 #pragma unroll
-          for (int nb = 0; nb < NB; ++nb) {
-            float alpha[2];
+          for (int c = 0; c < 2; ++c) {
+            float mx = top[c];
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              float mx = top[nb][c];
-#pragma unroll
-              for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
-              const float m_new = fmaxf(m[nb][c], mx);
-              alpha[c] = m_new == FAWS_NEG_INF ? 1.f : fast_exp2(m[nb][c] - m_new);
-              m[nb][c] = m_new;
-              l[nb][c] *= alpha[c];
-            }
-#pragma unroll
-            for (int gi = 0; gi < NG; ++gi)
-#pragma unroll
-              for (int c = 0; c < 4; ++c)
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt) o[nb][gi][mt][c] *= alpha[c & 1];
+            for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+            const float m_new = fmaxf(m[c], mx);
+            alpha[c] = m_new == FAWS_NEG_INF ? 1.f : fast_exp2(m[c] - m_new);
+            m[c] = m_new;
+            l[c] *= alpha[c];
           }
+#pragma unroll
+          for (int gi = 0; gi < NG; ++gi)
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+              for (int mt = 0; mt < MT; ++mt) o[gi][mt][c] *= alpha[c & 1];
         }
         // ---- weights, and values
 #pragma unroll
         for (int part = 0; part < 2; ++part) {
-          uint64_t pr[NB][2];  // [token g, g + 8], rows 2 t and 2 t + 1
+          uint64_t pr[2];  // [token g, g + 8], rows 2 t and 2 t + 1
 #pragma unroll
-          for (int nb = 0; nb < NB; ++nb) {
+          for (int half = 0; half < 2; ++half) {
+            float y[2];
+            unpack_f32x2(s[part][half], y[0], y[1]);
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              float y[2];
-              unpack_f32x2(s[part][nb][half], y[0], y[1]);
-#pragma unroll
-              for (int c = 0; c < 2; ++c) {
-                y[c] = fast_exp2(fmaf(y[c], f[nb][c], m[nb][c] == FAWS_NEG_INF ? 0.f : -m[nb][c]));
-                if (kMasked && (hidden[nb] >> (part * 4 + half * 2 + c) & 1u)) y[c] = 0.f;
-                l[nb][c] += y[c];
-              }
-              pr[nb][half] = pack_f32x2(y[0], y[1]);
+            for (int c = 0; c < 2; ++c) {
+              y[c] = fast_exp2(fmaf(y[c], f[c], m[c] == FAWS_NEG_INF ? 0.f : -m[c]));
+              if (kMasked && (hidden >> (part * 4 + half * 2 + c) & 1u)) y[c] = 0.f;
+              l[c] += y[c];
             }
+            pr[half] = pack_f32x2(y[0], y[1]);
           }
           uint64_t vs[2][NG];
           scales(1, part * 16 + krow, vs[0]);
@@ -942,22 +925,20 @@ __global__ void __launch_bounds__(CTA_THREADS, CTAS_PER_SM) cache_attn_kernel(co
             else vw[e][0] = vr[g];
           }
           // the weighted scales as operands, all of them before the products that wait for them
-          uint32_t pb[NB][NG][2];
+          uint32_t pb[NG][2];
 #pragma unroll
           for (int gi = 0; gi < NG; ++gi)
 #pragma unroll
-            for (int nb = 0; nb < NB; ++nb)
+            for (int half = 0; half < 2; ++half) {
+              float pv[2];
+              unpack_f32x2(mul_f32x2(pr[half], vs[half][gi]), pv[0], pv[1]);
+              if constexpr (kMasked) {  // a hidden token's scale may be anything
 #pragma unroll
-              for (int half = 0; half < 2; ++half) {
-                float pv[2];
-                unpack_f32x2(mul_f32x2(pr[nb][half], vs[half][gi]), pv[0], pv[1]);
-                if constexpr (kMasked) {  // a hidden token's scale may be anything
-#pragma unroll
-                  for (int c = 0; c < 2; ++c)
-                    if (hidden[nb] >> (part * 4 + half * 2 + c) & 1u) pv[c] = 0.f;
-                }
-                pb[nb][gi][half] = transpose8(pack2<__half>(pv[0], pv[1]));
+                for (int c = 0; c < 2; ++c)
+                  if (hidden >> (part * 4 + half * 2 + c) & 1u) pv[c] = 0.f;
               }
+              pb[gi][half] = transpose8(pack2<__half>(pv[0], pv[1]));
+            }
 #pragma unroll
           for (int gi = 0; gi < NG; ++gi) {
             // both tokens' half-words of the group; then with their bytes exchanged, which brings the next two nibbles
@@ -975,13 +956,10 @@ __global__ void __launch_bounds__(CTA_THREADS, CTAS_PER_SM) cache_attn_kernel(co
               const uint32_t y23 = __byte_perm(vw[2][gi >> 1], vw[3][gi >> 1], swapped);
               a1[0] = y01 & kLow; a1[1] = y01 & kHigh; a1[2] = y23 & kLow; a1[3] = y23 & kHigh;
             }
-#pragma unroll
-            for (int nb = 0; nb < NB; ++nb) {
-              mma_f16(o[nb][gi][0], a0, pb[nb][gi][0], pb[nb][gi][1]);
-              if constexpr (MT == 2) mma_f16(o[nb][gi][MT - 1], a1, pb[nb][gi][0], pb[nb][gi][1]);
-              mma_f16(o[nb][gi][0], less8, pb[nb][gi][0], pb[nb][gi][1]);
-              if constexpr (MT == 2) mma_f16(o[nb][gi][MT - 1], less8, pb[nb][gi][0], pb[nb][gi][1]);
-            }
+            mma_f16(o[gi][0], a0, pb[gi][0], pb[gi][1]);
+            if constexpr (MT == 2) mma_f16(o[gi][MT - 1], a1, pb[gi][0], pb[gi][1]);
+            mma_f16(o[gi][0], less8, pb[gi][0], pb[gi][1]);
+            if constexpr (MT == 2) mma_f16(o[gi][MT - 1], less8, pb[gi][0], pb[gi][1]);
           }
         }
       };
@@ -1003,25 +981,22 @@ __global__ void __launch_bounds__(CTA_THREADS, CTAS_PER_SM) cache_attn_kernel(co
 
       // ---- the four warps' parts
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
+      for (int c = 0; c < 2; ++c) {
+        float ls = l[c];
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          float ls = l[nb][c];
-#pragma unroll
-          for (int x = 4; x < 32; x <<= 1) ls += __shfl_xor_sync(0xffffffffu, ls, x);
-          if (g == 0) ml[warp * RT + nb * 8 + 2 * t + c] = make_float2(m[nb][c], ls);
-        }
-#pragma unroll
-        for (int gi = 0; gi < NG; ++gi)
-#pragma unroll
-          for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              const int row = nb * 8 + 2 * t + (c & 1);
-              const int d = D >= 32 ? 32 * gi + 4 * g + 2 * mt + (c >> 1) : 2 * g + (c >> 1);
-              so[row * L::kOutRow + d] = o[nb][gi][mt][c] * (c >> 1 ? 262144.f : 4194304.f);
-            }
+        for (int x = 4; x < 32; x <<= 1) ls += __shfl_xor_sync(0xffffffffu, ls, x);
+        if (g == 0) ml[warp * RT + 2 * t + c] = make_float2(m[c], ls);
       }
+#pragma unroll
+      for (int gi = 0; gi < NG; ++gi)
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const int row = 2 * t + (c & 1);
+            const int d = D >= 32 ? 32 * gi + 4 * g + 2 * mt + (c >> 1) : 2 * g + (c >> 1);
+            so[row * L::kOutRow + d] = o[gi][mt][c] * (c >> 1 ? 262144.f : 4194304.f);
+          }
       consumers_any(false);
       const bool begins = w.first == 0, ends = w.first + cnt == w.span.nt;
       const float* all = reinterpret_cast<const float*>(smem + L::out_off);
@@ -1207,7 +1182,6 @@ size_t cache_attn_workspace_bytes(int D) { return (size_t)shares_at_most() * (16
 cudaError_t launch_cache_attn(const CacheAttnParams& call, int dtype, cudaStream_t s) {
   CacheAttnParams p = call;
   p.grid = shares_at_most();
-  p.min_tiles = 1;
   p.vec_out = reinterpret_cast<uintptr_t>(p.out) % 8 == 0 && p.o_sb % 4 == 0 && p.o_sh % 4 == 0 && p.o_ss % 4 == 0;
   p.status = tc_status_word();
   return dtype == FAWS_FP16 ? launch_attn_t<__half>(p, s) : launch_attn_t<__nv_bfloat16>(p, s);

@@ -235,7 +235,7 @@ struct CacheAttnParams {
   int tiles_at_most;
   long long wait_cycles;
   // set by the launcher
-  int row_blocks, grid, min_tiles, vec_out;
+  int row_blocks, grid, vec_out;
   float* parts;       // workspace
   int* status;
 };
