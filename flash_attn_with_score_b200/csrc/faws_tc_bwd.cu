@@ -1043,6 +1043,9 @@ BwWs bwd_ws(int B, int Hq, int Hk, int M, int N, int D, bool fine) {
 // G times fewer and longer CTAs: taken where whole waves of those are expected to end no later.  bf16 Hq28 Hk4 S8192 D128, window
 // 1024, 4 sinks, dK and dV: 282 us a head at a time, 236 so; fp16 B2 H12 S1531 D64, window 300, 7 sinks, is better off without the
 // parts (57 us with the other kernels, 63 with).
+// Over 216 bf16 shapes (D 64 and 128; heads 12-12, 16-4, 28-4, 32-8, 8-1, 14-2; 512 to 8192 rows, batches of 1 to 4; windows 64 to
+// 1024; 0, 4, 300 sinks) the training step takes 1.8 % longer than with the better of the two ways for each shape, 11.7 % with
+// the heads always walked and 7.2 % with them never; at the worst 18 % (B4 Hq16 Hk4 S2048 D128, window 256, 4 sinks: 216 us, walked 183).
 struct WindowPlan {
   int loop, sink_tiles, ranges, parts, rows;  // parts: of a tile with sinks; rows: keys of these tiles
 };

@@ -11,7 +11,10 @@ template <typename T, int D>
 cudaError_t launch_t(const TcMaps& maps, const FwdParams& p, cudaStream_t s) {
   if (p.pack_m > 0 || p.n_splits > 1) return launch_fwd_s<T, D, kHookNone, true, kNoDrop, true, true>(maps, p, s);
   // 256-row CTAs, of two heads' rows where the group has an even number of them, against 128-row ones by the times that plain
-  // launches of as many key tiles are expected to take.
+  // launches of as many key tiles are expected to take.  Over 216 bf16 shapes (D 64 and 128; heads 12-12, 16-4, 28-4, 32-8, 8-1, 14-2; 512
+  // to 8192 rows, batches of 1 to 4; windows 64 to 1024; 0, 4, 300 sinks) that is 0.4 % longer than the better of the two, 8 % at
+  // the worst, where 256 rows throughout are 8 % longer and 128 rows twice as long; two heads to a CTA are 7.6 % shorter over the 108
+  // shapes with even groups, 2.6 % longer at the worst.
   FwdParams pp = p;
   pp.pair_heads = p.G % 2 == 0 ? 1 : 0;
   RowChoice c{(long long)p.B * p.Hq, p.m_begin, p.m_end, p.N, p.p_seq, p.causal, sm_count(), p.window, p.sinks};
