@@ -52,5 +52,5 @@ def test_other_threads_run_while_the_queue_is_full(name):
         other.join()
     torch.cuda.synchronize()
     assert took > 0.3, "the calls waited for the queue"
-    assert max(gaps) < 0.15, f"another thread stood still for {max(gaps):.2f} s of {took:.2f}"
+    assert max(gaps) < 0.5 * took, f"another thread stood still for {max(gaps):.2f} s of {took:.2f}"
     assert F.device_status() == 0
