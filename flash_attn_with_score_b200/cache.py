@@ -57,6 +57,9 @@ class KVCache4:
             raise AttributeError(f"a cache's {name} cannot be replaced: copy into its tensors, or make another cache")
         super().__setattr__(name, value)
 
+    def __delattr__(self, name):  # (nor without)
+        raise AttributeError(f"a cache's {name} cannot be deleted: calls go by its tensors' memory")
+
 
 def _batch(cache, page_table, lengths, B, rows):
     if not isinstance(cache, KVCache4):
